@@ -417,6 +417,113 @@ MC_API mc_status mc_sample_rows(const float* logits_dev, int32_t n_rows, int32_t
                                 float temperature, float top_p, float min_p, uint64_t seed,
                                 uint32_t round, uint32_t* tokens_dev, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Paged serving: long contexts in a 4-bit KV cache, whole prompts in one
+ * pass, page bookkeeping on the device.  No counterpart in the reference,
+ * whose caches are f32 or int8 and live on the host.
+ *
+ * Every pointer is device memory of `device`, every call is asynchronous on
+ * `stream` (a cudaStream_t as void*), allocates nothing and can be captured
+ * in a CUDA graph.  Index arrays are int32.  Strides count elements; the last
+ * axis of an activation is contiguous.  Sizes of zero are valid and do
+ * nothing.
+ */
+
+/* Activation types of the paged operators. */
+#define MC_ACT_F32 0
+#define MC_ACT_F16 1
+#define MC_ACT_BF16 2
+
+/* Block tables and slot maps of one step.  Request z holds kv_len[z] tokens
+ * and gets q_len[z] new ones (negative lengths count as 0).  Pages hold
+ * page_size tokens; the pages a request still lacks are taken from the top of
+ * the stack free_pages[0 .. *n_free), requests in order, and entered into
+ * table[z][table_width] in place.  Written: cu_q[n_requests + 1], the first
+ * new token of each request; for new token t its position and its slot (page
+ * * page_size + offset), for t from the last request's end to n_tokens
+ * position 0 and slot -1; new_len = kv_len + q_len; *n_free_out = *n_free
+ * minus the pages taken.  When the stack runs out *n_free_out is negative
+ * (the pages missing) and the tokens without a page get table entry and slot
+ * -1, as tokens beyond table_width pages get slot -1.  n_tokens must be at
+ * least the sum of q_len: tokens beyond it are not placed.  Inputs other than
+ * the table are left as they are, so a step can be planned again. */
+MC_API mc_status mc_paged_slots(const int32_t* kv_len, const int32_t* q_len, int32_t n_requests,
+                                int32_t* table, int32_t table_width, const int32_t* free_pages,
+                                int32_t n_free_pages, const int32_t* n_free, int32_t page_size,
+                                int32_t n_tokens, int32_t* cu_q, int32_t* positions,
+                                int32_t* slots, int32_t* new_len, int32_t* n_free_out,
+                                int32_t device, void* stream);
+
+/* Tables [positions][n_freq] of factor * cos and sin of position * freq, in
+ * f64, rounded once to f32 (freq: device memory). */
+MC_API mc_status mc_rope_table(const double* freq, int32_t n_freq, int32_t positions,
+                               double factor, float* cos_out, float* sin_out, int32_t device,
+                               void* stream);
+
+/* Rotary positions of q [n_tokens][n_heads][head_dim] and k (either may have
+ * no heads).  The first `rot` values of a head are rotated in pairs, (i, i +
+ * rot/2) or, interleaved, (2i, 2i + 1): y0 = x0 cos - x1 sin, y1 = x1 cos +
+ * x0 sin with row positions[t] of the tables [table_rows][rot/2]; the others
+ * are copied.  Arithmetic in f32, one rounding.  Outputs are contiguous, of
+ * the inputs' type, or for f32 inputs of any; an output may be its own
+ * contiguous input when the types agree.  A position outside the tables gives
+ * NaN. */
+MC_API mc_status mc_rope(const void* q, int64_t q_tok, int64_t q_head, int32_t n_heads,
+                         const void* k, int64_t k_tok, int64_t k_head, int32_t n_kv_heads,
+                         int32_t dtype, int32_t n_tokens, int32_t head_dim, int32_t rot,
+                         int32_t interleaved, const int32_t* positions, const float* cos_table,
+                         const float* sin_table, int32_t table_rows, void* q_out, void* k_out,
+                         int32_t out_dtype, int32_t device, void* stream);
+
+/* The 4-bit cache is a pool of pages [n_pages][n_kv_heads] of
+ * mc_kv4_page_bytes(head_dim) bytes each (0 for an unsupported head dim; 64
+ * and 128 are supported): 64 tokens of one key/value head, K and V as q4_0
+ * blocks of 32 values (quantized as the weights' q4_0: d = the value of
+ * largest size / -8, code = trunc(x / d + 8.5), value = (code - 8) f16(d)).
+ * A block that holds a non-finite value, or one beyond 8 x 65504, reads back
+ * non-finite.  Token slot s is token s % 64 of page s / 64. */
+MC_API int64_t mc_kv4_page_bytes(int32_t head_dim);
+/* k, v [n_tokens][n_kv_heads][head_dim] into their slots; slots outside the
+ * pool are skipped.  No two tokens of one call may share a slot. */
+MC_API mc_status mc_kv4_append(void* pool, int64_t n_pages, int32_t n_kv_heads, int32_t head_dim,
+                               const void* k, int64_t k_tok, int64_t k_head, const void* v,
+                               int64_t v_tok, int64_t v_head, int32_t dtype,
+                               const int32_t* slots, int32_t n_tokens, int32_t device,
+                               void* stream);
+/* The values of n_tokens slots, contiguous; slots outside the pool read as 0. */
+MC_API mc_status mc_kv4_read(const void* pool, int64_t n_pages, int32_t n_kv_heads,
+                             int32_t head_dim, const int32_t* slots, int32_t n_tokens, void* k_out,
+                             void* v_out, int32_t dtype, int32_t device, void* stream);
+
+/* Attention of the new tokens of n_requests requests over the 4-bit cache:
+ * softmax(scale q k^T) v, query head h reading key/value head h / (n_heads /
+ * n_kv_heads).  Rows cu_q[z] .. cu_q[z + 1] of q belong to request z and are
+ * the last of its kv_len[z] tokens (the cache holds them already): row j sees
+ * the tokens up to its own.  A row that sees none, and a row of no request,
+ * gives 0; so does a page whose table entry lies outside the pool count as
+ * not there.  q and out are f16 or bf16; out is contiguous. */
+MC_API mc_status mc_kv4_attention(const void* q, int64_t q_tok, int64_t q_head, int32_t dtype,
+                                  int32_t n_tokens, int32_t n_heads, const void* pool,
+                                  int64_t n_pages, int32_t n_kv_heads, int32_t head_dim,
+                                  const int32_t* table, int32_t table_width,
+                                  const int32_t* kv_len, const int32_t* cu_q,
+                                  int32_t n_requests, float scale, void* out, int32_t device,
+                                  void* stream);
+
+/* Attention over packed prompts: sequence z has queries cu_q[z] .. cu_q[z +
+ * 1] of q [n_q][n_heads][head_dim] and keys cu_k[z] .. cu_k[z + 1] of k and v
+ * [n_k][n_kv_heads][head_dim] (f16 or bf16, all of one type).  Causal: the
+ * sequence's queries are its last tokens, so query i sees the keys up to i +
+ * (keys - queries).  A row that sees no key, and a row of no sequence, gives
+ * 0.  out is contiguous, of q's type. */
+MC_API mc_status mc_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void* k,
+                                     int64_t k_tok, int64_t k_head, const void* v, int64_t v_tok,
+                                     int64_t v_head, int32_t dtype, int32_t n_q, int32_t n_k,
+                                     int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                                     const int32_t* cu_q, const int32_t* cu_k,
+                                     int32_t n_sequences, float scale, int32_t causal, void* out,
+                                     int32_t device, void* stream);
+
 MC_API size_t mc_last_error(char* buf, size_t cap);
 MC_API const char* mc_version(void);
 

@@ -12,4 +12,18 @@ from .model import (LLAMA2_70B, LLAMA3_8B, PRESETS, TINY, TINYLLAMA,  # noqa: F4
                     LlamaConfig, Linear, QTensor, Weights, quantize_int8_rows,
                     quantize_int8_tensor, synth_weights, synth_weights_torch)
 
+# The paged serving operators work on torch tensors: torch is imported with
+# the first of them that is used.
+_PAGED = ("PagedStep", "RopeScaling", "kv4_append", "kv4_attention", "kv4_pool", "kv4_read",
+          "paged_slots", "prompt_attention", "rope", "rope_frequencies", "rope_table")
+
+
+def __getattr__(name):
+    if name in _PAGED:
+        from . import paged
+        globals().update({n: getattr(paged, n) for n in _PAGED})
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
 __version__ = "0.1.0"

@@ -17,6 +17,7 @@ STATUS = {0: "MC_OK", -1: "MC_E_INVALID", -2: "MC_E_SHAPE", -3: "MC_E_DTYPE", -4
           -5: "MC_E_CUDA", -6: "MC_E_NCCL", -7: "MC_E_TIMEOUT", -8: "MC_E_CANCELLED",
           -9: "MC_E_NO_HEAD", -10: "MC_E_CAPACITY"}
 
+ACT_F32, ACT_F16, ACT_BF16 = 0, 1, 2  # activation types of the paged operators
 DTYPE_F32, DTYPE_I8_TENSOR, DTYPE_I8_ROW, DTYPE_Q4_0 = 0, 1, 2, 3
 MEM_HOST, MEM_DEVICE = 0, 1
 MODE_REFERENCE, MODE_GENERAL = 0, 1
@@ -35,6 +36,8 @@ EXPORTS = [
     "mc_ngram_draft_create", "mc_ngram_draft", "mc_ngram_draft_destroy", "mc_sample_rows",
     "mc_session_set_wait_timeout", "mc_session_create_mlp", "mc_kv_snapshot_take",
     "mc_kv_snapshot_tokens", "mc_kv_snapshot_destroy", "mc_spec_prime_cached",
+    "mc_paged_slots", "mc_rope_table", "mc_rope", "mc_kv4_page_bytes", "mc_kv4_append",
+    "mc_kv4_read", "mc_kv4_attention", "mc_prompt_attention",
 ]
 
 
@@ -142,6 +145,19 @@ def lib():
         "mc_ngram_draft_destroy": (i32, [vp]),
         "mc_sample_rows": (i32, [vp, i32, i32, C.c_float, C.c_float, C.c_float, C.c_uint64,
                                  C.c_uint32, vp, vp]),
+        "mc_paged_slots": (i32, [vp, vp, i32, vp, i32, vp, i32, vp, i32, i32, vp, vp, vp, vp, vp,
+                                 i32, vp]),
+        "mc_rope_table": (i32, [vp, i32, i32, C.c_double, vp, vp, i32, vp]),
+        "mc_rope": (i32, [vp, i64, i64, i32, vp, i64, i64, i32, i32, i32, i32, i32, i32, vp, vp,
+                          vp, i32, vp, vp, i32, i32, vp]),
+        "mc_kv4_page_bytes": (i64, [i32]),
+        "mc_kv4_append": (i32, [vp, i64, i32, i32, vp, i64, i64, vp, i64, i64, i32, vp, i32, i32,
+                                vp]),
+        "mc_kv4_read": (i32, [vp, i64, i32, i32, vp, i32, vp, vp, i32, i32, vp]),
+        "mc_kv4_attention": (i32, [vp, i64, i64, i32, i32, i32, vp, i64, i32, i32, vp, i32, vp,
+                                   vp, i32, C.c_float, vp, i32, vp]),
+        "mc_prompt_attention": (i32, [vp, i64, i64, vp, i64, i64, vp, i64, i64, i32, i32, i32, i32,
+                                      i32, i32, vp, vp, i32, C.c_float, i32, vp, i32, vp]),
         "mc_session_stream": (vp, [vp]),
         "mc_session_round_launches": (i32, [vp]),
         "mc_version": (C.c_char_p, []),

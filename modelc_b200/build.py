@@ -18,8 +18,9 @@ LIB = os.path.join(HERE, "libmodelc_cuda.so")
 # first-CTA start, release from the dependency wait and last-CTA end
 # (%globaltimer), plus per-phase times of the attention and tcgen05 kernels.
 TRACE_LIB = os.path.join(HERE, "libmodelc_cuda_trace.so")
-SOURCES = ["mc_kernels.cu", "mc_api.cu", "mc_drafters.cu", "mc_kvcache.cu"]
-HEADERS = ["mc_internal.cuh"]
+SOURCES = ["mc_kernels.cu", "mc_api.cu", "mc_drafters.cu", "mc_kvcache.cu", "mc_paged.cu",
+           "mc_kv4_attn.cu", "mc_prompt_attn.cu"]
+HEADERS = ["mc_internal.cuh", "mc_paged.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -43,7 +44,7 @@ def build(force: bool = False, verbose: bool = False, trace: bool = False) -> st
     lib = TRACE_LIB if trace else LIB
     if not force and not _stale(lib):
         return lib
-    cmd = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared",
+    cmd = [nvcc(), *ARCH, "-t", "0", "-O3", "-lineinfo", "-std=c++17", "-shared",
            "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
            *(["-DMC_TRACE"] if trace else []),
            "-I", os.path.join(ROOT, "include"),

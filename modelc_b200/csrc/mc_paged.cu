@@ -1,0 +1,527 @@
+// mc_paged.cu -- page bookkeeping, rotary positions and the 4-bit KV cache's
+// append and read back (include/modelc_cuda.h, the paged serving section).
+#include <algorithm>
+#include <atomic>
+
+#include "mc_paged.cuh"
+
+namespace mc {
+
+// ------------------------------------------------------------ device check
+constexpr int kMaxDevices = 64;
+static std::atomic<int> g_sms[kMaxDevices];  // SM count once checked, 0 before
+
+mc_status paged_device(int device) {
+  if (device < 0 || device >= kMaxDevices) return set_error(MC_E_INVALID, "bad device index");
+  if (!g_sms[device].load(std::memory_order_acquire)) {
+    int n = 0;
+    if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
+      cudaGetLastError();
+      return set_error(MC_E_CUDA, "no CUDA device");
+    }
+    if (device >= n) return set_error(MC_E_INVALID, "bad device index");
+    int major = 0, minor = 0, sms = 0;
+    MC_PCK(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
+    MC_PCK(cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device));
+    MC_PCK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+    if (major != 10 || minor != 0) return set_error(MC_E_CUDA, "not an sm_100 device");
+    g_sms[device].store(sms, std::memory_order_release);
+  }
+  int cur = -1;
+  MC_PCK(cudaGetDevice(&cur));
+  if (cur != device) MC_PCK(cudaSetDevice(device));
+  return MC_OK;
+}
+
+int paged_sms(int device) { return g_sms[device].load(std::memory_order_acquire); }
+
+// ---------------------------------------------- block tables and slot maps
+struct SlotArgs {
+  const int *kv_len, *q_len;
+  int* table;
+  const int *free_pages, *n_free;
+  int *cu_q, *positions, *slots, *new_len, *n_free_out;
+  int B, width, page, tokens, n_pages_free;
+};
+
+// Every block scans all requests, a chunk of one request per thread at a
+// time, and places the tokens of its own stretch of the output that belong
+// to the chunk: one launch, no exchange between blocks.  A fresh page is
+// written into the table by the token that opens it (the one at a multiple
+// of the page size), so tables cost no loop of their own.  The scan reads
+// 8 B bytes from L2 in every block; what bounds the call is its latency.
+constexpr int kSlotThreads = 1024;
+
+__global__ void __launch_bounds__(kSlotThreads) k_paged_slots(const SlotArgs a) {
+  __shared__ int s_cu[kSlotThreads], s_start[kSlotThreads], s_kv[kSlotThreads];
+  __shared__ int w_tok[32], w_pg[32];
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  const int per = (int)(((long long)a.tokens + gridDim.x - 1) / gridDim.x);
+  const long long lo = (long long)blockIdx.x * per;
+  const long long hi = min((long long)a.tokens, lo + per);
+  const int n_free = max(*a.n_free, 0);
+  long long base_tok = 0, base_pg = 0;
+  if (blockIdx.x == 0 && tid == 0) a.cu_q[0] = 0;
+  for (int z0 = 0; z0 < a.B; z0 += kSlotThreads) {
+    const int z = z0 + tid;
+    int kv = 0, q = 0;
+    if (z < a.B) {
+      kv = max(a.kv_len[z], 0);
+      q = max(a.q_len[z], 0);
+    }
+    const int have = min((kv + a.page - 1) / a.page, a.width);
+    const int need = min((kv + q + a.page - 1) / a.page, a.width);
+    int tok = q, pg = need - have;  // inclusive sums over the chunk
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(~0u, tok, o), y = __shfl_up_sync(~0u, pg, o);
+      if (lane >= o) tok += x, pg += y;
+    }
+    if (lane == 31) w_tok[wid] = tok, w_pg[wid] = pg;
+    __syncthreads();
+    if (wid == 0) {
+      int x = w_tok[lane], y = w_pg[lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(~0u, x, o), v = __shfl_up_sync(~0u, y, o);
+        if (lane >= o) x += u, y += v;
+      }
+      w_tok[lane] = x, w_pg[lane] = y;
+    }
+    __syncthreads();
+    if (wid) tok += w_tok[wid - 1], pg += w_pg[wid - 1];
+    const int n_tok = w_tok[31], n_pg = w_pg[31];
+    s_cu[tid] = tok - q;  // tokens of the chunk before this request
+    s_start[tid] = pg - (need - have) - have;
+    s_kv[tid] = kv;
+    if (blockIdx.x == 0 && z < a.B) {
+      a.cu_q[z + 1] = (int)(base_tok + tok);
+      a.new_len[z] = kv + q;
+    }
+    __syncthreads();
+    // this chunk's tokens are [base_tok, base_tok + n_tok)
+    const long long t0 = max(lo, base_tok), t1 = min(hi, base_tok + n_tok);
+    const int nz = min(kSlotThreads, a.B - z0);
+    for (long long t = t0 + tid; t < t1; t += kSlotThreads) {
+      const int i = (int)(t - base_tok);
+      int l = 0, r = nz;  // the last request that starts at or before token i
+      while (r - l > 1) {
+        const int m = (l + r) >> 1;
+        if (s_cu[m] <= i) l = m;
+        else r = m;
+      }
+      const int kvl = s_kv[l], pos = kvl + i - s_cu[l], j = pos / a.page;
+      int page = -1;
+      if (j < a.width) {
+        int* entry = a.table + (size_t)(z0 + l) * a.width + j;
+        if (j >= (kvl + a.page - 1) / a.page) {
+          const long long nth = (long long)n_free - 1 - (base_pg + s_start[l] + j);
+          if (nth >= 0 && nth < a.n_pages_free) page = a.free_pages[nth];
+          if (pos % a.page == 0) *entry = page;
+        } else {
+          page = *entry;
+        }
+      }
+      a.positions[t] = pos;
+      a.slots[t] = page < 0 ? -1 : page * a.page + pos % a.page;
+    }
+    base_tok += n_tok;
+    base_pg += n_pg;
+    __syncthreads();
+  }
+  for (long long t = max(lo, base_tok) + tid; t < hi; t += kSlotThreads) {
+    a.positions[t] = 0;
+    a.slots[t] = -1;
+  }
+  if (blockIdx.x == 0 && tid == 0) *a.n_free_out = (int)(*a.n_free - base_pg);
+}
+
+// -------------------------------------------------------- rotary positions
+// cos and sin of position * frequency in 64 bits, rounded once: an angle of
+// 1e5 radians held in 32 bits would be off by 4e-3.
+__global__ void k_rope_table(const double* freq, int n, int positions, double factor, float* cs,
+                             float* sn) {
+  const long long total = (long long)positions * n;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
+       i += (long long)gridDim.x * blockDim.x) {
+    double s, c;
+    sincos((double)(i / n) * freq[i % n], &s, &c);
+    cs[i] = (float)(c * factor);
+    sn[i] = (float)(s * factor);
+  }
+}
+
+struct RopeArgs {
+  const void *q, *k;
+  void *qo, *ko;
+  long long q_tok, q_head, k_tok, k_head;  // input strides, elements
+  const int* positions;
+  const float *cs, *sn;
+  int T, H, Hk, D, rot, max_pos, HG;
+};
+
+template <typename T, int V>
+struct __align__(sizeof(T) * V <= 16 ? sizeof(T) * V : 16) Pack {
+  T x[V];
+};
+
+// A unit is 2V values of one head: V pairs, or 2V values behind the rotated
+// part that are copied.  A thread keeps one (token, unit) for HPT heads, so
+// its cos and sin are read once for all of them; consecutive threads take
+// consecutive units, then heads.
+template <typename TI, typename TO, int V, int HPT, bool HALF>
+__global__ void __launch_bounds__(256) k_rope(const RopeArgs a) {
+  const unsigned U = a.D / (2 * V);
+  const unsigned idx = blockIdx.x * 256u + threadIdx.x;
+  const unsigned u = idx % U, rest = idx / U, hg = rest % a.HG, t = rest / a.HG;
+  if (t >= (unsigned)a.T) return;
+  const int half = a.rot / 2, RU = half / V;
+  const bool turn = u < (unsigned)RU;
+  // where the unit's two groups of V values start
+  const int e0 = !turn ? a.rot + (u - RU) * 2 * V : HALF ? u * V : u * 2 * V;
+  const int e1 = turn && HALF ? e0 + half : e0 + V;
+  const int pos = a.positions[t];
+  const bool known = pos >= 0 && pos < a.max_pos;
+  Pack<TI, V> x0[HPT], x1[HPT];
+#pragma unroll
+  for (int i = 0; i < HPT; ++i) {
+    const int h = hg + i * a.HG;
+    if (h < a.H + a.Hk) {
+      const TI* p = h < a.H ? (const TI*)a.q + t * a.q_tok + h * a.q_head
+                            : (const TI*)a.k + t * a.k_tok + (h - a.H) * a.k_head;
+      x0[i] = *(const Pack<TI, V>*)(p + e0);
+      x1[i] = *(const Pack<TI, V>*)(p + e1);
+    }
+  }
+  Pack<float, V> c, s;
+  if (turn && known) {
+    c = *(const Pack<float, V>*)(a.cs + (size_t)pos * half + u * V);
+    s = *(const Pack<float, V>*)(a.sn + (size_t)pos * half + u * V);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      c.x[j] = turn ? __int_as_float(0x7fffffff) : 1.f;  // no such position: NaN
+      s.x[j] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < HPT; ++i) {
+    const int h = hg + i * a.HG;
+    if (h >= a.H + a.Hk) break;
+    Pack<TO, V> y0, y1;
+    if (!turn) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        y0.x[j] = from_f<TO>(to_f(x0[i].x[j]));
+        y1.x[j] = from_f<TO>(to_f(x1[i].x[j]));
+      }
+    } else if (HALF) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float p = to_f(x0[i].x[j]), r = to_f(x1[i].x[j]);
+        y0.x[j] = from_f<TO>(p * c.x[j] - r * s.x[j]);
+        y1.x[j] = from_f<TO>(r * c.x[j] + p * s.x[j]);
+      }
+    } else {  // pair j of the unit: values 2j and 2j + 1 of its 2V
+      float y[2 * V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float p = to_f(2 * j < V ? x0[i].x[(2 * j) % V] : x1[i].x[(2 * j) % V]);
+        const float r = to_f(2 * j + 1 < V ? x0[i].x[(2 * j + 1) % V] : x1[i].x[(2 * j + 1) % V]);
+        y[2 * j] = p * c.x[j] - r * s.x[j];
+        y[2 * j + 1] = r * c.x[j] + p * s.x[j];
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        y0.x[j] = from_f<TO>(y[j]);
+        y1.x[j] = from_f<TO>(y[V + j]);
+      }
+    }
+    TO* o = h < a.H ? (TO*)a.qo + ((size_t)t * a.H + h) * a.D
+                    : (TO*)a.ko + ((size_t)t * a.Hk + (h - a.H)) * a.D;
+    *(Pack<TO, V>*)(o + e0) = y0;
+    *(Pack<TO, V>*)(o + e1) = y1;
+  }
+}
+
+template <typename TI, typename TO, int V, int HPT>
+static cudaError_t run_rope(RopeArgs a, bool half, cudaStream_t s) {
+  a.HG = (a.H + a.Hk + HPT - 1) / HPT;
+  const long long n = (long long)a.T * a.HG * (a.D / (2 * V));
+  const unsigned grid = (unsigned)((n + 255) / 256);
+  if (half) k_rope<TI, TO, V, HPT, true><<<grid, 256, 0, s>>>(a);
+  else k_rope<TI, TO, V, HPT, false><<<grid, 256, 0, s>>>(a);
+  return cudaGetLastError();
+}
+
+template <typename TI, typename TO>
+static cudaError_t run_rope_types(const RopeArgs& a, bool half, int vec, bool wide, cudaStream_t s) {
+  if (vec >= 4) {
+    return wide ? run_rope<TI, TO, 4, 4>(a, half, s) : run_rope<TI, TO, 4, 1>(a, half, s);
+  }
+  return run_rope<TI, TO, 1, 1>(a, half, s);
+}
+
+// ------------------------------------------------ append to the 4-bit pages
+struct AppendArgs {
+  const void *k, *v;
+  long long k_tok, k_head, v_tok, v_head;  // strides, elements
+  const int* slots;
+  uint8_t* pool;
+  int T, Hk, n_slots;
+};
+
+// W = D/8 lanes take one row (a token's K or V of one head); lane w holds the
+// values w, w + W, ... of its word.  A block's first value of largest size is
+// the maximum of (size, 31 - place, sign) over the W lanes.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) k_kv4_append(const AppendArgs a) {
+  constexpr int W = D / 8, NB = D / 32, PB = 32 / W;  // PB: values of a block in one lane
+  const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / W;
+  const int w = threadIdx.x % W;
+  const long long n_rows = 2ll * a.T * a.Hk;
+  const bool live = row < n_rows;
+  const int kv = live ? (int)(row % 2) : 0;
+  const int h = live ? (int)((row / 2) % a.Hk) : 0;
+  const long long t = live ? row / 2 / a.Hk : 0;
+  const int slot = live ? a.slots[t] : -1;
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  if (slot >= 0 && slot < a.n_slots) {
+    const T* p = kv ? (const T*)a.v + t * a.v_tok + h * a.v_head
+                    : (const T*)a.k + t * a.k_tok + h * a.k_head;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f(p[i * W + w]);
+  }
+  uint32_t word = 0;
+  float mine = 0.f;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    unsigned long long key = 0;
+#pragma unroll
+    for (int i = 0; i < PB; ++i) {
+      const uint32_t bits = __float_as_uint(x[b * PB + i]);
+      const unsigned long long c = ((unsigned long long)(bits & 0x7fffffffu) << 6) |
+                                   (unsigned)((31 - (i * W + w)) << 1) | (bits >> 31);
+      key = c > key ? c : key;
+    }
+#pragma unroll
+    for (int o = W / 2; o; o >>= 1) {
+      const unsigned long long c = __shfl_xor_sync(~0u, key, o, W);
+      key = c > key ? c : key;
+    }
+    const float top = __uint_as_float((uint32_t)(key >> 6) | ((uint32_t)(key & 1) << 31));
+    const float d = __fdiv_rn(top, -8.f);
+    const float inv = d != 0.f ? __fdiv_rn(1.f, d) : 0.f;
+#pragma unroll
+    for (int i = 0; i < PB; ++i) {
+      // the product and the sum are rounded one by one, as the rule says
+      const float y = __fadd_rn(__fmul_rn(x[b * PB + i], inv), 8.5f);
+      const int code = (int)fminf(fmaxf(y, 0.f), 15.f);
+      word |= (uint32_t)code << (4 * kv4_nib(b * PB + i));
+    }
+    if (w == b) mine = d;
+  }
+  if (slot < 0 || slot >= a.n_slots) return;
+  const int s = slot % kKv4Page;
+  uint8_t* page = a.pool + ((size_t)(slot / kKv4Page) * a.Hk + h) * kv4_page_bytes(D);
+  ((uint32_t*)(page + kv * 32 * D + s * (D / 2)))[kv4_word_at<D>(s, w)] = word;
+  if (w < NB)
+    ((__half*)(page + 64 * D + kv * 4 * D))[kv4_scale_at(s, w, NB)] = __float2half_rn(mine);
+}
+
+struct ReadArgs {
+  const uint8_t* pool;
+  const int* slots;
+  void *k, *v;  // [T][Hk][D]
+  int T, Hk, n_slots;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256) k_kv4_read(const ReadArgs a) {
+  constexpr int W = D / 8, NB = D / 32, PB = 32 / W;
+  const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / W;
+  const int w = threadIdx.x % W;
+  if (row >= 2ll * a.T * a.Hk) return;
+  const int kv = (int)(row % 2), h = (int)((row / 2) % a.Hk);
+  const long long t = row / 2 / a.Hk;
+  const int slot = a.slots[t];
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  if (slot >= 0 && slot < a.n_slots) {
+    const int s = slot % kKv4Page;
+    const uint8_t* page = a.pool + ((size_t)(slot / kKv4Page) * a.Hk + h) * kv4_page_bytes(D);
+    const uint32_t word = ((const uint32_t*)(page + kv * 32 * D + s * (D / 2)))[kv4_word_at<D>(s, w)];
+    const __half* sc = (const __half*)(page + 64 * D + kv * 4 * D);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      x[i] = (float)((int)((word >> (4 * kv4_nib(i))) & 15) - 8) *
+             __half2float(sc[kv4_scale_at(s, i / PB, NB)]);
+  }
+  T* o = (T*)(kv ? a.v : a.k) + (t * a.Hk + h) * D;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i * W + w] = from_f<T>(x[i]);
+}
+
+template <template <typename, int> class F, int D, typename... A>
+static cudaError_t by_type(int dtype, A&&... args) {
+  if (dtype == MC_ACT_F32) return F<float, D>::run(args...);
+  if (dtype == MC_ACT_F16) return F<__half, D>::run(args...);
+  return F<__nv_bfloat16, D>::run(args...);
+}
+template <typename T, int D>
+struct Append {
+  static cudaError_t run(const AppendArgs& a, cudaStream_t s) {
+    const long long n = 2ll * a.T * a.Hk * (D / 8);
+    k_kv4_append<T, D><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a);
+    return cudaGetLastError();
+  }
+};
+template <typename T, int D>
+struct Read {
+  static cudaError_t run(const ReadArgs& a, cudaStream_t s) {
+    const long long n = 2ll * a.T * a.Hk * (D / 8);
+    k_kv4_read<T, D><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a);
+    return cudaGetLastError();
+  }
+};
+
+}  // namespace mc
+
+using namespace mc;
+
+// ------------------------------------------------------------------ C entries
+extern "C" mc_status mc_paged_slots(const int32_t* kv_len, const int32_t* q_len, int32_t n_requests,
+                                    int32_t* table, int32_t table_width, const int32_t* free_pages,
+                                    int32_t n_free_pages, const int32_t* n_free, int32_t page_size,
+                                    int32_t n_tokens, int32_t* cu_q, int32_t* positions,
+                                    int32_t* slots, int32_t* new_len, int32_t* n_free_out,
+                                    int32_t device, void* stream) {
+  if (n_requests < 0 || n_tokens < 0 || table_width < 0 || n_free_pages < 0)
+    return set_error(MC_E_INVALID, "negative size");
+  if (page_size <= 0) return set_error(MC_E_SHAPE, "page size must be positive");
+  if (!n_free || !cu_q || !n_free_out || (n_requests > 0 && (!kv_len || !q_len || !new_len)) ||
+      (n_requests > 0 && table_width > 0 && !table) || (n_free_pages > 0 && !free_pages) ||
+      (n_tokens > 0 && (!positions || !slots)))
+    return set_error(MC_E_INVALID, "null pointer");
+  MC_PCKS(paged_device(device));
+  SlotArgs a{kv_len, q_len, table, free_pages, n_free, cu_q, positions, slots, new_len, n_free_out,
+             n_requests, table_width, page_size, n_tokens, n_free_pages};
+  const int grid = std::max(1, std::min(paged_sms(device), (n_tokens + kSlotThreads - 1) / kSlotThreads));
+  k_paged_slots<<<grid, kSlotThreads, 0, (cudaStream_t)stream>>>(a);
+  MC_PCK(cudaGetLastError());
+  return MC_OK;
+}
+
+extern "C" mc_status mc_rope_table(const double* freq, int32_t n_freq, int32_t positions,
+                                   double factor, float* cos_out, float* sin_out, int32_t device,
+                                   void* stream) {
+  if (n_freq <= 0 || positions <= 0) return set_error(MC_E_SHAPE, "empty table");
+  if (!freq || !cos_out || !sin_out) return set_error(MC_E_INVALID, "null pointer");
+  MC_PCKS(paged_device(device));
+  const long long n = (long long)positions * n_freq;
+  const int grid = (int)std::min<long long>((n + 255) / 256, 8ll * paged_sms(device));
+  k_rope_table<<<grid, 256, 0, (cudaStream_t)stream>>>(freq, n_freq, positions, factor, cos_out, sin_out);
+  MC_PCK(cudaGetLastError());
+  return MC_OK;
+}
+
+static size_t act_size(int t) { return t == MC_ACT_F32 ? 4 : 2; }
+
+extern "C" mc_status mc_rope(const void* q, int64_t q_tok, int64_t q_head, int32_t n_heads,
+                             const void* k, int64_t k_tok, int64_t k_head, int32_t n_kv_heads,
+                             int32_t dtype, int32_t n_tokens, int32_t head_dim, int32_t rot,
+                             int32_t interleaved, const int32_t* positions, const float* cos_table,
+                             const float* sin_table, int32_t table_rows, void* q_out, void* k_out,
+                             int32_t out_dtype, int32_t device, void* stream) {
+  if (n_tokens < 0 || n_heads < 0 || n_kv_heads < 0) return set_error(MC_E_INVALID, "negative size");
+  if (head_dim <= 0 || head_dim % 2 || rot <= 0 || rot % 2 || rot > head_dim)
+    return set_error(MC_E_SHAPE, "rot must be even and positive, at most the (even) head dim");
+  if (dtype < 0 || dtype > 2 || out_dtype < 0 || out_dtype > 2 ||
+      (out_dtype != dtype && dtype != MC_ACT_F32))
+    return set_error(MC_E_DTYPE, "output type: the input's, or any for f32 inputs");
+  if (table_rows <= 0) return set_error(MC_E_SHAPE, "empty table");
+  if (n_tokens == 0 || n_heads + n_kv_heads == 0) return MC_OK;
+  if (!positions || !cos_table || !sin_table || (n_heads && (!q || !q_out)) ||
+      (n_kv_heads && (!k || !k_out)))
+    return set_error(MC_E_INVALID, "null pointer");
+  if ((long long)n_tokens * (n_heads + n_kv_heads) * (head_dim / 2) >= (1ll << 31) * 4)
+    return set_error(MC_E_CAPACITY, "too many values for one call");
+  MC_PCKS(paged_device(device));
+  RopeArgs a{q, k, q_out, k_out, q_tok, q_head, k_tok, k_head, positions, cos_table, sin_table,
+             n_tokens, n_heads, n_kv_heads, head_dim, rot, table_rows, 0};
+  // Groups of four values where all sizes, strides and addresses allow the
+  // aligned vector access they need, single values otherwise.
+  const size_t vi = 4 * act_size(dtype), vo = 4 * act_size(out_dtype);
+  const bool vec = (rot / 2) % 4 == 0 && head_dim % 8 == 0 && aligned(cos_table, 16) && aligned(sin_table, 16) &&
+                   (!n_heads || (aligned(q, vi) && aligned(q_out, vo) && q_tok % 4 == 0 && q_head % 4 == 0)) &&
+                   (!n_kv_heads || (aligned(k, vi) && aligned(k_out, vo) && k_tok % 4 == 0 && k_head % 4 == 0));
+  if (!vec && (long long)n_tokens * (n_heads + n_kv_heads) * (head_dim / 2) >= (1ll << 31))
+    return set_error(MC_E_CAPACITY, "too many values for one call");
+  // Four heads a thread once that still fills the GPU.
+  const bool wide = (long long)n_tokens * (n_heads + n_kv_heads) * head_dim >= (1ll << 22);
+  cudaStream_t s = (cudaStream_t)stream;
+  const int v = vec ? 4 : 1;
+  const bool half = !interleaved;
+  cudaError_t e;
+  if (dtype == MC_ACT_F32)
+    e = out_dtype == MC_ACT_F32   ? run_rope_types<float, float>(a, half, v, wide, s)
+        : out_dtype == MC_ACT_F16 ? run_rope_types<float, __half>(a, half, v, wide, s)
+                                  : run_rope_types<float, __nv_bfloat16>(a, half, v, wide, s);
+  else if (dtype == MC_ACT_F16)
+    e = run_rope_types<__half, __half>(a, half, v, wide, s);
+  else
+    e = run_rope_types<__nv_bfloat16, __nv_bfloat16>(a, half, v, wide, s);
+  MC_PCK(e);
+  return MC_OK;
+}
+
+static mc_status check_pool(const void* pool, int64_t n_pages, int32_t n_kv_heads, int32_t head_dim) {
+  if (head_dim != 64 && head_dim != 128) return set_error(MC_E_SHAPE, "head dim must be 64 or 128");
+  if (n_kv_heads <= 0 || n_pages < 0) return set_error(MC_E_SHAPE, "bad pool shape");
+  if (n_pages * kKv4Page > 0x7fffffffll) return set_error(MC_E_CAPACITY, "slots pass 31 bits");
+  if (n_pages && (!pool || !aligned(pool, 16)))
+    return set_error(MC_E_INVALID, "pool must be 16-byte aligned");
+  return MC_OK;
+}
+
+extern "C" int64_t mc_kv4_page_bytes(int32_t head_dim) {
+  return head_dim == 64 || head_dim == 128 ? kv4_page_bytes(head_dim) : 0;
+}
+
+extern "C" mc_status mc_kv4_append(void* pool, int64_t n_pages, int32_t n_kv_heads, int32_t head_dim,
+                                   const void* k, int64_t k_tok, int64_t k_head, const void* v,
+                                   int64_t v_tok, int64_t v_head, int32_t dtype,
+                                   const int32_t* slots, int32_t n_tokens, int32_t device,
+                                   void* stream) {
+  MC_PCKS(check_pool(pool, n_pages, n_kv_heads, head_dim));
+  if (dtype < 0 || dtype > 2) return set_error(MC_E_DTYPE, "unknown type");
+  if (n_tokens < 0) return set_error(MC_E_INVALID, "negative size");
+  if (n_tokens == 0) return MC_OK;
+  if (!k || !v || !slots) return set_error(MC_E_INVALID, "null pointer");
+  if ((long long)n_tokens * n_kv_heads * head_dim / 4 >= (1ll << 39))
+    return set_error(MC_E_CAPACITY, "too many values for one call");
+  MC_PCKS(paged_device(device));
+  AppendArgs a{k, v, k_tok, k_head, v_tok, v_head, slots, (uint8_t*)pool, n_tokens, n_kv_heads,
+               (int)(n_pages * kKv4Page)};
+  MC_PCK(head_dim == 128 ? (by_type<Append, 128>(dtype, a, (cudaStream_t)stream))
+                         : (by_type<Append, 64>(dtype, a, (cudaStream_t)stream)));
+  return MC_OK;
+}
+
+extern "C" mc_status mc_kv4_read(const void* pool, int64_t n_pages, int32_t n_kv_heads,
+                                 int32_t head_dim, const int32_t* slots, int32_t n_tokens, void* k_out,
+                                 void* v_out, int32_t dtype, int32_t device, void* stream) {
+  MC_PCKS(check_pool(pool, n_pages, n_kv_heads, head_dim));
+  if (dtype < 0 || dtype > 2) return set_error(MC_E_DTYPE, "unknown type");
+  if (n_tokens < 0) return set_error(MC_E_INVALID, "negative size");
+  if (n_tokens == 0) return MC_OK;
+  if (!k_out || !v_out || !slots) return set_error(MC_E_INVALID, "null pointer");
+  MC_PCKS(paged_device(device));
+  ReadArgs a{(const uint8_t*)pool, slots, k_out, v_out, n_tokens, n_kv_heads, (int)(n_pages * kKv4Page)};
+  MC_PCK(head_dim == 128 ? (by_type<Read, 128>(dtype, a, (cudaStream_t)stream))
+                         : (by_type<Read, 64>(dtype, a, (cudaStream_t)stream)));
+  return MC_OK;
+}

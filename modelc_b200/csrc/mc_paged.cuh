@@ -1,0 +1,88 @@
+// mc_paged.cuh -- what the paged serving operators share: activation types,
+// the 4-bit page format and the host-side checks of their C entry points.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "mc_internal.cuh"
+#include "modelc_cuda.h"
+
+namespace mc {
+
+mc_status set_error(mc_status st, const char* msg);  // mc_api.cu
+
+// Makes `device` current after checking once that it is an sm_100 device.
+mc_status paged_device(int device);
+int paged_sms(int device);  // its SM count (after paged_device)
+
+#define MC_PCK(call)                                                          \
+  do {                                                                        \
+    cudaError_t e_ = (call);                                                  \
+    if (e_ != cudaSuccess)                                                    \
+      return ::mc::set_error(e_ == cudaErrorMemoryAllocation ? MC_E_OOM : MC_E_CUDA, \
+                             cudaGetErrorString(e_));                         \
+  } while (0)
+#define MC_PCKS(expr)             \
+  do {                            \
+    mc_status s_ = (expr);        \
+    if (s_ != MC_OK) return s_;   \
+  } while (0)
+
+inline bool aligned(const void* p, size_t n) { return ((uintptr_t)p % n) == 0; }
+
+// ---------------------------------------------------------------------------
+// The 4-bit page.  64 tokens of one key/value head in 72 D bytes (D = 64 or
+// 128): K codes (64 rows of D/2 bytes), V codes, K scales, V scales (f16).
+// Values follow the q4_0 rule of the weights: per 32 consecutive values
+// d = (the value of largest size, first on ties) / -8, code = trunc(x/d + 8.5)
+// in 0..15, value = (code - 8) f16(d).
+//
+// A row of D codes is W = D/8 words; value d sits in word d % W, nibble
+// nib(d / W).  nib(2p) = p and nib(2p + 1) = p + 4, so that
+// (word >> 8(p/2)) & (0x000f000f << 4(p%2)) is an f16 pair of the values
+// (2p W + w, (2p + 1) W + w), both in one block of 32: the codes read as f16
+// subnormals, code * 2^-24 (2^-20 for odd p), with no conversion.
+// Tokens of D = 128 whose bit 1 is set hold the two 32-byte halves of a row
+// swapped: the four rows a warp reads at once then lie in different banks.
+// Scales are stored in the order in which the attention's lanes use them:
+// [8 groups of 8 tokens][4 t][D/32 blocks][2 e], entry (t, b, e) for token
+// kv4_token(2t + e) of the group.
+// ---------------------------------------------------------------------------
+constexpr int kKv4Page = 64;
+__host__ __device__ constexpr int kv4_page_bytes(int D) { return 72 * D; }
+// Tensor-core column n of a group of 8 tokens holds token kv4_token(n), its own inverse.
+__host__ __device__ inline int kv4_token(int n) { return n < 4 ? n : n ^ 1; }
+__host__ __device__ inline int kv4_nib(int i) { return (i >> 1) + 4 * (i & 1); }
+// Index of block b of token s (0..63) in a page's K or V scales.
+__host__ __device__ inline int kv4_scale_at(int s, int b, int NB) {
+  const int n = kv4_token(s & 7);
+  return (((s >> 3) * 4 + (n >> 1)) * NB + b) * 2 + (n & 1);
+}
+// Word index of logical word w in the row of token s.
+template <int D>
+__host__ __device__ inline int kv4_word_at(int s, int w) {
+  return D == 128 ? w ^ ((s & 2) << 2) : w;
+}
+
+// ------------------------------------------------------------ type helpers
+template <typename T>
+__device__ __forceinline__ float to_f(T x);
+template <>
+__device__ __forceinline__ float to_f<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f<__half>(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f(float x);
+template <>
+__device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+}  // namespace mc
