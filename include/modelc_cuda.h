@@ -501,14 +501,17 @@ MC_API mc_status mc_kv4_read(const void* pool, int64_t n_pages, int32_t n_kv_hea
  * the last of its kv_len[z] tokens (the cache holds them already): row j sees
  * the tokens up to its own.  A row that sees none, and a row of no request,
  * gives 0; so does a page whose table entry lies outside the pool count as
- * not there.  q and out are f16 or bf16; out is contiguous. */
+ * not there.  q and out are f16 or bf16; out is contiguous.  The workspace
+ * (16-byte aligned, of the size that mc_kv4_attention_workspace gives, 0 on
+ * an error) needs no clearing and is free again when the call has run. */
+MC_API int64_t mc_kv4_attention_workspace(int32_t n_requests, int32_t head_dim, int32_t device);
 MC_API mc_status mc_kv4_attention(const void* q, int64_t q_tok, int64_t q_head, int32_t dtype,
                                   int32_t n_tokens, int32_t n_heads, const void* pool,
                                   int64_t n_pages, int32_t n_kv_heads, int32_t head_dim,
                                   const int32_t* table, int32_t table_width,
                                   const int32_t* kv_len, const int32_t* cu_q,
-                                  int32_t n_requests, float scale, void* out, int32_t device,
-                                  void* stream);
+                                  int32_t n_requests, float scale, void* out, void* workspace,
+                                  int64_t workspace_bytes, int32_t device, void* stream);
 
 /* Attention over packed prompts: sequence z has queries cu_q[z] .. cu_q[z +
  * 1] of q [n_q][n_heads][head_dim] and keys cu_k[z] .. cu_k[z + 1] of k and v

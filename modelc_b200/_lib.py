@@ -37,7 +37,7 @@ EXPORTS = [
     "mc_session_set_wait_timeout", "mc_session_create_mlp", "mc_kv_snapshot_take",
     "mc_kv_snapshot_tokens", "mc_kv_snapshot_destroy", "mc_spec_prime_cached",
     "mc_paged_slots", "mc_rope_table", "mc_rope", "mc_kv4_page_bytes", "mc_kv4_append",
-    "mc_kv4_read", "mc_kv4_attention", "mc_prompt_attention",
+    "mc_kv4_read", "mc_kv4_attention_workspace", "mc_kv4_attention", "mc_prompt_attention",
 ]
 
 
@@ -155,7 +155,8 @@ def lib():
                                 vp]),
         "mc_kv4_read": (i32, [vp, i64, i32, i32, vp, i32, vp, vp, i32, i32, vp]),
         "mc_kv4_attention": (i32, [vp, i64, i64, i32, i32, i32, vp, i64, i32, i32, vp, i32, vp,
-                                   vp, i32, C.c_float, vp, i32, vp]),
+                                   vp, i32, C.c_float, vp, vp, i64, i32, vp]),
+        "mc_kv4_attention_workspace": (i64, [i32, i32, i32]),
         "mc_prompt_attention": (i32, [vp, i64, i64, vp, i64, i64, vp, i64, i64, i32, i32, i32, i32,
                                       i32, i32, vp, vp, i32, C.c_float, i32, vp, i32, vp]),
         "mc_session_stream": (vp, [vp]),

@@ -85,4 +85,46 @@ __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// ------------------------------------------------- asynchronous copies
+__device__ __forceinline__ uint32_t sm_ptr(const void* p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(sm_ptr(b)), "r"(n) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(sm_ptr(b)), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(sm_ptr(b)) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(sm_ptr(b)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// Waits for the phase with this parity, a bounded number of rounds (each try
+// suspends the thread for a while by itself; far above any copy's time).
+__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity) {
+  for (int i = 0; i < (1 << 22); ++i)
+    if (bar_try(b, parity)) return true;
+  return false;
+}
+// `bytes` (a multiple of 16) from global to shared memory, both 16-byte
+// aligned, counted on an mbarrier of this block.
+__device__ __forceinline__ void copy_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* b) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          sm_ptr(dst)),
+      "l"(src), "r"(bytes), "r"(sm_ptr(b))
+      : "memory");
+}
+
 }  // namespace mc

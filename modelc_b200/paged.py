@@ -238,12 +238,13 @@ def kv4_attention(q, pool, table, kv_len, cu_q, scale: float | None = None):
         raise ValueError(f"table: [{B}, width] is wanted")
     Hk = pool.shape[1]
     out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
+    ws = torch.empty(lib().mc_kv4_attention_workspace(B, D, dev.index), dtype=torch.uint8, device=dev)
     qs = q.stride()
     check(lib().mc_kv4_attention(q.data_ptr(), qs[0], qs[1], _ACT[q.dtype], T, H, pool.data_ptr(),
                                  pool.shape[0], Hk, D, _index(table, "table", dev), table.shape[1],
                                  _index(kv_len, "kv_len", dev), _index(cu_q, "cu_q", dev, (B + 1,)),
                                  B, D ** -0.5 if scale is None else scale, out.data_ptr(),
-                                 dev.index, _stream(dev)))
+                                 ws.data_ptr(), ws.numel(), dev.index, _stream(dev)))
     return out
 
 

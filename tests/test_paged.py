@@ -537,11 +537,12 @@ def test_kv4_append_and_read_refuse(status, args):
 
 @pytest.mark.parametrize("status,args", [
     (-2, dict(D=80)), (-2, dict(H=5)), (-3, dict(dt=0)), (-1, dict(T=-1)), (-1, dict(q=None)),
-    (-1, dict(scale=math.inf)), (-10, dict(pages=1 << 26)), (-1, dict(pool=C.c_void_p(4104)))])
+    (-1, dict(scale=math.inf)), (-10, dict(pages=1 << 26)), (-1, dict(pool=C.c_void_p(4104))),
+    (-1, dict(ws=None))])
 def test_kv4_attention_refuses(status, args):
-    d = dict(D=128, H=4, dt=2, T=3, q=P, scale=0.1, pages=9, pool=P) | args
+    d = dict(D=128, H=4, dt=2, T=3, q=P, scale=0.1, pages=9, pool=P, ws=P) | args
     assert mb.lib().mc_kv4_attention(d["q"], 512, 128, d["dt"], d["T"], d["H"], d["pool"], d["pages"], 2, d["D"], P,
-                                     4, P, P, 1, d["scale"], P, 0, None) == status
+                                     4, P, P, 1, d["scale"], P, d["ws"], 0, 0, None) == status
 
 
 @pytest.mark.parametrize("status,args", [
