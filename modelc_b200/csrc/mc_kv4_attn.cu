@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps<NP>, 1) k_kv4(const Kv4Args a) 
     };
 
     for (; page < end; ++page) {
-      if (!failed && !bar_wait(&s_full[wid][st], phase)) failed = true;
+      if (!failed && !warp_wait(&s_full[wid][st], phase)) failed = true;
       if (!failed && s_there[wid][st]) {
         const uint8_t* pg = ring + st * PB;
 #pragma unroll 1

@@ -110,12 +110,23 @@ __device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
       : "memory");
   return done != 0;
 }
-// Waits for the phase with this parity, a bounded number of rounds (each try
-// suspends the thread for a while by itself; far above any copy's time).
+// Waits for the phase with this parity, two seconds at most: far above any
+// copy's or product's time, so it runs out only when something else failed.
 __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity) {
-  for (int i = 0; i < (1 << 22); ++i)
+  for (int i = 0; i < 64; ++i)
     if (bar_try(b, parity)) return true;
+  unsigned long long t0, t1;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  do {
+    for (int i = 0; i < 64; ++i)
+      if (bar_try(b, parity)) return true;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1));
+  } while (t1 - t0 < 2000000000ull);
   return false;
+}
+// The same for a whole warp: true where no lane's wait ran out.
+__device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity) {
+  return __all_sync(~0u, bar_wait(b, parity));
 }
 // `bytes` (a multiple of 16) from global to shared memory, both 16-byte
 // aligned, counted on an mbarrier of this block.

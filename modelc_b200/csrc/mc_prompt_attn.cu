@@ -1,9 +1,33 @@
 // mc_prompt_attn.cu -- attention over whole packed prompts.
+//
+// O = softmax(scale Q K^T) V per sequence and head, one pass over the keys.
+// A block takes 256 query rows of one head as two tiles of 128 and walks the
+// keys in tiles of 128:
+//   - one thread loads Q once and K, V tiles through a shared-memory ring
+//     (cp.async.bulk.tensor, 128-byte swizzle);
+//   - one thread issues tcgen05.mma: S = Q K^T of a tile into tensor memory,
+//     and O += P V with P read from tensor memory, where it took the place of
+//     S;
+//   - two groups of four warps, one per tile, turn S into P: a thread owns a
+//     row, so maxima and sums need no exchange.
+// While one tile's rows are in the softmax the tensor cores work on the
+// other tile.  Scores, statistics and O are f32; P is rounded to the inputs'
+// type.  The reference of the exponentials follows the running maximum only
+// when that has grown by more than 2^8: O is then rescaled in tensor memory.
+#include <cuda.h>
 #include <math.h>
+
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 #include "mc_paged.cuh"
 
 namespace mc {
+
+constexpr int kPromptRows = 128;  // rows of a query tile, keys of a key tile
+constexpr int kPromptThreads = 384;
+constexpr float kPromptGrow = 8.f;  // log2 growth of the maximum that is let pass
 
 struct PromptArgs {
   const void *q, *k, *v;  // [Tq][H][D], [Tk][Hk][D] with strides (elements)
@@ -14,50 +38,520 @@ struct PromptArgs {
   float scale;
 };
 
-// One warp per (row, head): scores with a lane per key, then the values with
-// a lane per dimension.
-template <typename T, int D>
-__global__ void __launch_bounds__(32) k_prompt_simple(const PromptArgs a) {
-  constexpr int NB = D / 32;
-  __shared__ float s_q[D];
-  const int lane = threadIdx.x, t = blockIdx.x, h = blockIdx.y;
-  int z = -1;
-  for (int i = 0; i < a.B; ++i)
-    if (t >= a.cu_q[i] && t < a.cu_q[i + 1]) z = i;
-  float o[NB] = {}, m = -INFINITY, l = 0.f;
-  if (z >= 0) {
-    const T* q = (const T*)a.q + t * a.q_tok + h * a.q_head;
-    for (int i = lane; i < D; i += 32) s_q[i] = to_f(q[i]) * a.scale;
-    __syncwarp();
-    const int k0 = a.cu_k[z], L = min(a.cu_k[z + 1], a.Tk) - k0;
-    const int n = a.causal ? min(L, a.cu_k[z + 1] - k0 - (a.cu_q[z + 1] - 1 - t)) : L;
-    const int hk = h / (a.H / a.Hk);
-    for (int j0 = 0; j0 < n; j0 += 32) {
-      const int j = j0 + lane;
-      float x = -INFINITY;
-      if (j < n) {
-        const T* k = (const T*)a.k + (k0 + j) * a.k_tok + hk * a.k_head;
-        x = 0.f;
-        for (int i = 0; i < D; ++i) x += to_f(k[i]) * s_q[i];
-      }
-      float top = x;
-      for (int f = 16; f; f >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, f));
-      const float mn = fmaxf(m, top);
-      const float c = m == -INFINITY ? 0.f : __expf(m - mn);
-      const float e = x > -INFINITY ? __expf(x - mn) : (x != x ? x : 0.f);
-      m = mn;
-      l = l * c + e;
-      for (int b = 0; b < NB; ++b) o[b] *= c;
-      for (int i = 0; i < min(32, n - j0); ++i) {
-        const float p = __shfl_sync(~0u, e, i);
-        const T* v = (const T*)a.v + (k0 + j0 + i) * a.v_tok + hk * a.v_head;
-        for (int b = 0; b < NB; ++b) o[b] += p * to_f(v[b * 32 + lane]);
-      }
+template <int D>
+struct PromptCfg {
+  static constexpr int Tile = kPromptRows * D * 2;         // bytes of a Q, K or V tile
+  static constexpr int Half = kPromptRows * 128;           // of 64 of its columns
+  static constexpr int Slots = D == 128 ? 5 : 10;          // K and V tiles in the ring
+  static constexpr int Smem = (2 + Slots) * Tile + 1024;   // + alignment to the swizzle atoms
+  static constexpr uint32_t O = 256;                       // tensor memory columns: S 0, S 1, O 0, O 1
+};
+
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t pred;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(pred));
+  return pred;
+}
+// 64 columns x 128 rows at (column x, head h, token t)
+__device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* m, int x, int h, int t, uint64_t* b) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(sm_ptr(dst)),
+      "l"(m), "r"(x), "r"(h), "r"(t), "r"(sm_ptr(b))
+      : "memory");
+}
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo) {
+  // start, leading and stride byte offsets in 16-byte units (8 rows of 128
+  // bytes are 1024), descriptor version 1, 128-byte swizzle
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* b) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(sm_ptr(b))
+               : "memory");
+}
+#define MC_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define MC_I8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+// 32 columns of the warp's 32 lanes
+__device__ __forceinline__ void tm_load(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : MC_R8(r, 0), MC_R8(r, 8), MC_R8(r, 16), MC_R8(r, 24)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tm_store(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::MC_I8(r, 0),
+      MC_I8(r, 8), MC_I8(r, 16), MC_I8(r, 24), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tm_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  uint32_t x;
+  memcpy(&x, &h, 4);
+  return x;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  uint32_t x;
+  memcpy(&x, &h, 4);
+  return x;
+}
+
+struct PromptWork {
+  int q0, n_q;     // first query row of the block's 256 and how many the sequence has from there
+  int k0, L;       // first key, keys
+  int shift;       // a row i of the 256 sees the keys below i + shift (causal)
+  int ok;          // there is work
+};
+
+// The block's rows: tiles are counted over the sequences, the last ones
+// first, since under a causal mask they have the most keys.  One warp.
+__device__ __forceinline__ void prompt_work(const PromptArgs& a, int index, PromptWork* w) {
+  const int lane = threadIdx.x & 31;
+  int total = 0;
+  for (int z0 = 0; z0 < a.B; z0 += 32) {
+    const int z = z0 + lane;
+    int n = 0;
+    if (z < a.B) {
+      const int c0 = min(max(a.cu_q[z], 0), a.Tq);
+      n = max(min(a.cu_q[z + 1], a.Tq) - c0, 0);
     }
-    for (int f = 16; f; f >>= 1) l += __shfl_xor_sync(~0u, l, f);
+    total += __reduce_add_sync(~0u, (n + 255) / 256);
   }
+  if (lane == 0) w->ok = 0;
+  __syncwarp();
+  const int want = total - 1 - index;
+  if (want < 0) return;
+  int seen = 0;
+  for (int z0 = 0; z0 < a.B; z0 += 32) {
+    const int z = z0 + lane;
+    int n = 0, c0 = 0;
+    if (z < a.B) {
+      c0 = min(max(a.cu_q[z], 0), a.Tq);
+      n = max(min(a.cu_q[z + 1], a.Tq) - c0, 0);
+    }
+    const int mine = (n + 255) / 256;
+    int inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(~0u, inc, o);
+      if (lane >= o) inc += x;
+    }
+    const int first = seen + inc - mine;
+    if (want >= first && want < first + mine) {
+      const int r = (want - first) * 256;
+      const int k0 = min(max(a.cu_k[z], 0), a.Tk), k1 = max(min(a.cu_k[z + 1], a.Tk), k0);
+      w->q0 = c0 + r;
+      w->n_q = n - r;
+      w->k0 = k0;
+      w->L = k1 - k0;
+      w->shift = a.causal ? (a.cu_k[z + 1] - a.cu_k[z]) - n + r + 1 : 1 << 30;
+      w->ok = 1;
+    }
+    seen += __shfl_sync(~0u, inc, 31);
+    if (seen > want) break;
+  }
+  __syncwarp();
+}
+
+// One row again, with a lane per key and then per column, over its own keys
+// alone: for rows whose result is not finite, since a product of a hidden
+// key's weight 0 with its NaN or infinity is not 0.
+template <typename T, int D>
+__device__ __noinline__ void prompt_row(const PromptArgs& a, int t, int h, int k0, int n) {
+  constexpr int NB = D / 32;
+  const int lane = threadIdx.x & 31;
+  const T* q = (const T*)a.q + t * a.q_tok + h * a.q_head;
+  const int hk = h / (a.H / a.Hk);
+  const T* kp = (const T*)a.k + hk * a.k_head;
+  const T* vp = (const T*)a.v + hk * a.v_head;
+  float o[NB] = {}, m = -INFINITY, l = 0.f;
+  for (int j0 = 0; j0 < n; j0 += 32) {
+    const int j = j0 + lane;
+    float x = -INFINITY;
+    if (j < n) {
+      const T* k = kp + (long long)(k0 + j) * a.k_tok;
+      x = 0.f;
+      for (int i = 0; i < D; ++i) x += to_f(k[i]) * to_f(q[i]);
+      x *= a.scale;
+    }
+    float top = x;
+    for (int f = 16; f; f >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, f));
+    const float mn = fmaxf(m, top);
+    const float c = m == -INFINITY ? 0.f : __expf(m - mn);
+    const float e = x > -INFINITY ? __expf(x - mn) : (x != x ? x : 0.f);
+    m = mn;
+    l = l * c + e;
+    for (int b = 0; b < NB; ++b) o[b] *= c;
+    for (int i = 0; i < min(32, n - j0); ++i) {
+      const float p = __shfl_sync(~0u, e, i);
+      const T* v = vp + (long long)(k0 + j0 + i) * a.v_tok;
+      for (int b = 0; b < NB; ++b) o[b] += p * to_f(v[b * 32 + lane]);
+    }
+  }
+  for (int f = 16; f; f >>= 1) l += __shfl_xor_sync(~0u, l, f);
   T* out = (T*)a.out + ((size_t)t * a.H + h) * D;
   for (int b = 0; b < NB; ++b) out[b * 32 + lane] = from_f<T>(l != 0.f ? o[b] / l : 0.f);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPromptThreads, 1)
+    k_prompt(const PromptArgs a, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+             const __grid_constant__ CUtensorMap mv) {
+  using C = PromptCfg<D>;
+  constexpr int NH = D / 64;  // 64-column halves of a tile
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (sm_ptr(smem_raw) & 1023u)) & 1023u);
+  uint8_t *sq = smem, *ring = smem + 2 * C::Tile;
+  __shared__ __align__(8) uint64_t b_q, b_full[C::Slots], b_empty[C::Slots], b_s[2], b_p[2], b_pv[2], b_fix;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_fail;
+  __shared__ PromptWork s_work;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int head = blockIdx.x % a.H, index = blockIdx.x / a.H;
+
+  // rows of no sequence are 0: each block clears its share
+  {
+    const int end = min(max(a.B ? a.cu_q[a.B] : 0, 0), a.Tq);
+    const long long n = (long long)(a.Tq - end) * a.H * (D / 8);
+    uint4* z = (uint4*)((T*)a.out + (size_t)end * a.H * D);
+    for (long long i = (long long)blockIdx.x * kPromptThreads + tid; i < n; i += (long long)gridDim.x * kPromptThreads)
+      z[i] = make_uint4(0, 0, 0, 0);
+  }
+  if (warp == 0) prompt_work(a, index, &s_work);
+  if (tid == 32) {
+    bar_init(&b_q, 1);
+    for (int i = 0; i < C::Slots; ++i) bar_init(&b_full[i], 1), bar_init(&b_empty[i], 1);
+    for (int i = 0; i < 2; ++i) bar_init(&b_s[i], 1), bar_init(&b_p[i], 4), bar_init(&b_pv[i], 1);
+    bar_init(&b_fix, 1);
+    s_fail = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  if (!s_work.ok) return;
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm_ptr(&s_tmem)), "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tm_before();
+  __syncthreads();
+  tm_after();
+  const uint32_t tmem = s_tmem;
+  const PromptWork w = s_work;
+  const int hk = head / (a.H / a.Hk);
+  // keys that the last row of a tile sees, and its key tiles
+  int lim[2], n_t[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int rows = min(max(w.n_q - t * kPromptRows, 0), kPromptRows);
+    lim[t] = rows ? min(max(t * kPromptRows + rows - 1 + w.shift, 0), w.L) : 0;
+    n_t[t] = (lim[t] + kPromptRows - 1) / kPromptRows;
+  }
+  const int n_max = max(n_t[0], n_t[1]);
+  // keys of the last key tile, where the sequence or the mask ends inside it
+  const int tail = max(lim[0], lim[1]) - (n_max - 1) * kPromptRows;
+  const bool fix = n_max > 0 && tail % 16 != 0;
+
+  // Of the block's 384 x 168 registers the softmax's two groups of warps take
+  // 216 a thread and the third group keeps 72: 256 x 216 + 128 x 72 is the same.
+  if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+  if (warp == 9) {
+    // ----------------------------------------------------------- loads
+    bool ok = true;
+    if (n_max > 0) {
+      if (lane == 0) {
+        const int tiles = n_t[1] ? 2 : 1;
+        bar_expect(&b_q, tiles * C::Tile);
+        for (int t = 0; t < tiles; ++t)
+          for (int h = 0; h < NH; ++h)
+            load_tile(sq + t * C::Tile + h * C::Half, &mq, h * 64, head, w.q0 + t * kPromptRows, &b_q);
+      }
+      for (int i = 0; i < 2 * n_max && ok; ++i) {  // K 0, V 0, K 1, V 1, ...
+        const int slot = i % C::Slots, use = i / C::Slots;
+        if (use) ok = warp_wait(&b_empty[slot], (use - 1) & 1);
+        if (lane == 0 && ok) {
+          bar_expect(&b_full[slot], C::Tile);
+          for (int h = 0; h < NH; ++h)
+            load_tile(ring + slot * C::Tile + h * C::Half, i & 1 ? &mv : &mk, h * 64, hk,
+                      w.k0 + (i >> 1) * kPromptRows, &b_full[slot]);
+        }
+        __syncwarp();
+      }
+      if (fix && ok) {
+        // the last V tile's rows behind the last key, as far as a product's
+        // 16 keys reach, become 0: what lies there is not this sequence's
+        const int i = 2 * n_max - 1, slot = i % C::Slots;
+        ok = warp_wait(&b_full[slot], (i / C::Slots) & 1);
+        if (ok)
+          for (int r = tail; r < (tail + 15) / 16 * 16; ++r)
+            for (int x = lane; x < NH * 8; x += 32)
+              *(uint4*)(ring + slot * C::Tile + (x / 8) * C::Half + r * 128 + (x % 8) * 16) = make_uint4(0, 0, 0, 0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) bar_arrive(&b_fix);
+      }
+      if (!ok && lane == 0) s_fail = 1;
+    }
+  } else if (warp == 8) {
+    // -------------------------------------------------------- products
+    if (n_max > 0) {
+      bool ok = warp_wait(&b_q, 0);
+      // f32 accumulator; type of A and B; B of P V has its columns contiguous; N; M
+      constexpr uint32_t F = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+      const uint32_t id_s = (1u << 4) | (F << 7) | (F << 10) | ((a.scale < 0.f ? 1u : 0u) << 13) |
+                            ((uint32_t)(kPromptRows >> 3) << 17) | ((uint32_t)(kPromptRows >> 4) << 24);
+      const uint32_t id_o = (1u << 4) | (F << 7) | (F << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) |
+                            ((uint32_t)(kPromptRows >> 4) << 24);
+      const bool one = elect_one();
+      auto scores = [&](int t, int j) {
+        const int slot = (2 * j) % C::Slots;
+        if (one) {
+          const uint64_t da = smem_desc(sm_ptr(sq + t * C::Tile), 16), db = smem_desc(sm_ptr(ring + slot * C::Tile), 16);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint64_t off = (k % 4) * 2 + (k / 4) * (C::Half >> 4);
+            mma_ss(tmem + t * 128, da + off, db + off, id_s, k > 0);
+          }
+          mma_commit(&b_s[t]);
+        }
+        __syncwarp();
+      };
+      auto values = [&](int t, int j) {
+        const int slot = (2 * j + 1) % C::Slots;
+        if (one) {
+          const uint64_t db = smem_desc(sm_ptr(ring + slot * C::Tile), C::Half);
+          const int steps = min(8, (lim[t] - j * kPromptRows + 15) / 16);
+          for (int k = 0; k < steps; ++k)
+            mma_ts(tmem + C::O + t * D, tmem + t * 128 + k * 8, db + k * (2048 >> 4), id_o, j > 0 || k > 0);
+          mma_commit(&b_pv[t]);
+        }
+        __syncwarp();
+      };
+      ok = ok && warp_wait(&b_full[0], 0);
+      if (ok) {
+        tm_after();
+        for (int t = 0; t < 2; ++t)
+          if (n_t[t]) scores(t, 0);
+        if (one) mma_commit(&b_empty[0]);
+      }
+      for (int j = 0; j < n_max && ok; ++j) {
+        const int vi = 2 * j + 1, ki = 2 * j + 2;
+        bool have_k = false;
+        ok = warp_wait(&b_full[vi % C::Slots], (vi / C::Slots) & 1);
+        if (j == n_max - 1 && fix) ok = ok && warp_wait(&b_fix, 0);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (j >= n_t[t]) continue;
+          ok = ok && warp_wait(&b_p[t], j & 1);
+          if (!ok) break;
+          tm_after();
+          values(t, j);
+          if (j + 1 < n_t[t]) {
+            if (!have_k) {
+              ok = warp_wait(&b_full[ki % C::Slots], (ki / C::Slots) & 1);
+              have_k = true;
+            }
+            if (ok) scores(t, j + 1);
+          }
+        }
+        if (ok && one) {
+          mma_commit(&b_empty[vi % C::Slots]);
+          if (have_k) mma_commit(&b_empty[ki % C::Slots]);
+        }
+        __syncwarp();
+      }
+      if (!ok && lane == 0) s_fail = 1;
+    }
+  } else if (warp < 8) {
+    // --------------------------------------------------------- softmax
+    const int t = warp >> 2, row = t * kPromptRows + (warp & 3) * 32 + lane;
+    const uint32_t base = tmem + ((uint32_t)(warp & 3) << 21);  // the warp's 32 lanes
+    const uint32_t ts = base + t * 128, to = base + C::O + t * D;
+    const int n = n_t[t];
+    const int see = row < w.n_q ? min(max(row + w.shift, 0), w.L) : 0;  // keys of this row
+    const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      ok = ok && warp_wait(&b_s[t], j & 1);
+      if (!ok) break;
+      tm_after();
+      uint32_t s[128];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tm_load(ts + i * 32, s + i * 32);
+      tm_wait_ld();
+      const int left = see - j * kPromptRows;  // visible columns
+      if (!__all_sync(~0u, left >= kPromptRows)) {
+#pragma unroll
+        for (int i = 0; i < 128; ++i) s[i] = i < left ? s[i] : 0xff800000u;
+      }
+      float top = __uint_as_float(s[0]);
+#pragma unroll
+      for (int i = 1; i < 128; ++i) top = fmaxf(top, __uint_as_float(s[i]));
+      const bool grown = (top - m) * c > kPromptGrow;  // also from -inf
+      if (__any_sync(~0u, grown)) {
+        const float mn = grown ? top : m;
+        if (j > 0) {  // rescale O once the last product is in it
+          const float f = mn == m ? 1.f : m == -INFINITY ? 0.f : ex2f((m - mn) * c);
+          l *= f;
+          ok = warp_wait(&b_pv[t], (j - 1) & 1);
+          if (!ok) break;
+          tm_after();
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            uint32_t o[32];
+            tm_load(to + i * 32, o);
+            tm_wait_ld();
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+            tm_store(to + i * 32, o);
+          }
+        }
+        m = mn;
+      }
+      const float mc = m == -INFINITY ? 0.f : m * c;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t p[32];
+#pragma unroll
+        for (int x = 0; x < 32; ++x) {
+          const float e0 = ex2f(fmaf(__uint_as_float(s[i * 64 + 2 * x]), c, -mc));
+          const float e1 = ex2f(fmaf(__uint_as_float(s[i * 64 + 2 * x + 1]), c, -mc));
+          sum += e0 + e1;
+          p[x] = pack2<T>(e0, e1);
+        }
+        tm_store(ts + i * 32, p);
+      }
+      l += sum;
+      tm_wait_st();
+      tm_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&b_p[t]);
+    }
+    // ------------------------------------------------------- the result
+    if (n > 0) ok = ok && warp_wait(&b_pv[t], (n - 1) & 1);
+    if (!ok) s_fail = 1;
+    tm_after();
+    const float f = l != 0.f ? 1.f / l : 0.f;
+    const bool live = row < w.n_q;
+    T* out = (T*)a.out + ((size_t)(w.q0 + row) * a.H + head) * D;
+    bool bad = false;
+    if (n > 0 && ok) {
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        uint32_t o[32], y[16];
+        tm_load(to + i * 32, o);
+        tm_wait_ld();
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          // a row without keys has l = 0 and P = 0: its O may still hold NaN
+          const float y0 = __uint_as_float(o[2 * x]) * f, y1 = __uint_as_float(o[2 * x + 1]) * f;
+          bad |= !(fabsf(y0) <= 3e38f) || !(fabsf(y1) <= 3e38f);
+          y[x] = pack2<T>(y0, y1);
+        }
+        if (live)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            *(uint4*)(out + i * 32 + x * 8) = make_uint4(y[4 * x], y[4 * x + 1], y[4 * x + 2], y[4 * x + 3]);
+      }
+    } else if (live) {  // no keys; or a wait ran out
+      const uint32_t y = ok ? 0u : 0x7fff7fffu;
+      for (int x = 0; x < D / 8; ++x) *(uint4*)(out + x * 8) = make_uint4(y, y, y, y);
+    }
+    __syncwarp();
+    for (unsigned again = __ballot_sync(~0u, bad && live); again; again &= again - 1) {
+      const int r = __ffs(again) - 1;
+      prompt_row<T, D>(a, w.q0 + t * kPromptRows + (warp & 3) * 32 + r, head, w.k0, __shfl_sync(~0u, see, r));
+    }
+    tm_before();
+  }
+  __syncthreads();
+  if (s_fail && warp == 9 ) {  // leave no copy in flight
+    warp_wait(&b_q, 0);
+    for (int i = max(0, 2 * n_max - C::Slots); i < 2 * n_max; ++i) warp_wait(&b_full[i % C::Slots], (i / C::Slots) & 1);
+  }
+  if (warp == 8) {
+    tm_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// ------------------------------------------------------------- host side
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiled encode_tiled() {
+  static std::atomic<EncodeTiled> fn{nullptr};
+  EncodeTiled f = fn.load(std::memory_order_acquire);
+  if (!f) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) == cudaSuccess &&
+        r == cudaDriverEntryPointSuccess)
+      fn.store(f = (EncodeTiled)p, std::memory_order_release);
+  }
+  return f;
+}
+// boxes of 64 columns x 1 head x 128 tokens of [n][heads][D]
+static bool head_map(CUtensorMap* m, bool bf16, const void* p, int D, int heads, int n, long long tok, long long head) {
+  const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)n};
+  const cuuint64_t strides[2] = {(cuuint64_t)head * 2, (cuuint64_t)tok * 2};
+  const cuuint32_t box[3] = {64, 1, kPromptRows}, step[3] = {1, 1, 1};
+  EncodeTiled f = encode_tiled();
+  return f && f(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, (void*)p, dims,
+                strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+template <typename T, int D>
+static cudaError_t run_prompt(const PromptArgs& a, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+                              unsigned grid, cudaStream_t s) {
+  static std::atomic<unsigned long long> ready{0};  // devices whose attribute is set
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (!(ready.load(std::memory_order_acquire) >> dev & 1)) {
+    e = cudaFuncSetAttribute(k_prompt<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptCfg<D>::Smem);
+    if (e != cudaSuccess) return e;
+    ready.fetch_or(1ull << dev, std::memory_order_acq_rel);
+  }
+  k_prompt<T, D><<<grid, kPromptThreads, PromptCfg<D>::Smem, s>>>(a, q, k, v);
+  return cudaGetLastError();
 }
 
 }  // namespace mc
@@ -80,18 +574,34 @@ extern "C" mc_status mc_prompt_attention(const void* q, int64_t q_tok, int64_t q
   if (!isfinite(scale)) return set_error(MC_E_INVALID, "scale must be finite");
   if (n_q == 0) return MC_OK;
   if (!q || !out || !cu_q || !cu_k || (n_k && (!k || !v))) return set_error(MC_E_INVALID, "null pointer");
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) ||
+      (q_tok | q_head | k_tok | k_head | v_tok | v_head) % 8)
+    return set_error(MC_E_INVALID, "rows must be 16-byte aligned");
+  if (q_tok < 0 || q_head < 0 || k_tok < 0 || k_head < 0 || v_tok < 0 || v_head < 0)
+    return set_error(MC_E_INVALID, "negative stride");
+  const long long blocks = ((long long)(n_q + 255) / 256 + n_sequences) * n_heads;
+  if (blocks > 0x7fffffffll) return set_error(MC_E_CAPACITY, "too many rows for one call");
   MC_PCKS(paged_device(device));
+  cudaStream_t s = (cudaStream_t)stream;
+  if (n_k == 0 || n_sequences == 0) {  // no row sees a key
+    MC_PCK(cudaMemsetAsync(out, 0, (size_t)n_q * n_heads * head_dim * 2, s));
+    return MC_OK;
+  }
   PromptArgs a{q, k, v, q_tok, q_head, k_tok, k_head, v_tok, v_head, out, cu_q, cu_k, n_q, n_k,
                n_heads, n_kv_heads, n_sequences, causal, scale};
-  dim3 grid(n_q, n_heads);
-  cudaStream_t s = (cudaStream_t)stream;
-  if (dtype == MC_ACT_F16) {
-    if (head_dim == 128) k_prompt_simple<__half, 128><<<grid, 32, 0, s>>>(a);
-    else k_prompt_simple<__half, 64><<<grid, 32, 0, s>>>(a);
-  } else {
-    if (head_dim == 128) k_prompt_simple<__nv_bfloat16, 128><<<grid, 32, 0, s>>>(a);
-    else k_prompt_simple<__nv_bfloat16, 64><<<grid, 32, 0, s>>>(a);
-  }
-  MC_PCK(cudaGetLastError());
+  CUtensorMap mq, mk, mv;
+  const bool bf = dtype == MC_ACT_BF16;
+  if (!head_map(&mq, bf, q, head_dim, n_heads, n_q, q_tok, q_head) ||
+      !head_map(&mk, bf, k, head_dim, n_kv_heads, n_k, k_tok, k_head) ||
+      !head_map(&mv, bf, v, head_dim, n_kv_heads, n_k, v_tok, v_head))
+    return set_error(MC_E_CUDA, "the driver refused a tensor map of these strides");
+  cudaError_t e;
+  if (bf)
+    e = head_dim == 128 ? run_prompt<__nv_bfloat16, 128>(a, mq, mk, mv, (unsigned)blocks, s)
+                        : run_prompt<__nv_bfloat16, 64>(a, mq, mk, mv, (unsigned)blocks, s);
+  else
+    e = head_dim == 128 ? run_prompt<__half, 128>(a, mq, mk, mv, (unsigned)blocks, s)
+                        : run_prompt<__half, 64>(a, mq, mk, mv, (unsigned)blocks, s);
+  MC_PCK(e);
   return MC_OK;
 }

@@ -40,6 +40,16 @@ def _heads(t: torch.Tensor, name: str, device) -> torch.Tensor:
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
+def _rows16(t: torch.Tensor):
+    """f16 or bf16 rows whose every head starts at a multiple of 16 bytes (a
+    copy where they do not), with their token and head strides."""
+    s = t.stride()
+    if s[0] <= 0 or s[1] <= 0 or (s[0] | s[1]) % 8 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        return t, t.shape[1] * t.shape[2], t.shape[2]
+    return t, s[0], s[1]
+
+
 def _gpu(t: torch.Tensor, name: str):
     if not t.is_cuda:
         raise ValueError(f"{name}: a CUDA tensor is wanted")
@@ -261,14 +271,14 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, scale: float | None = None, causa
         raise ValueError("q, k, v: one type, f16 or bf16, is wanted")
     if k.shape != v.shape or k.shape[2] != D:
         raise ValueError("k, v: one shape, with q's head dim, is wanted")
+    (q, qt, qh), (k, kt, kh), (v, vt, vh) = _rows16(q), _rows16(k), _rows16(v)
     cu_k = cu_q if cu_k is None else cu_k
     B = cu_q.shape[0] - 1
     if B < 0:
         raise ValueError("cu_q: [sequences + 1] is wanted")
     out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
-    qs, ks, vs = q.stride(), k.stride(), v.stride()
-    check(lib().mc_prompt_attention(q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
-                                    v.data_ptr(), vs[0], vs[1], _ACT[q.dtype], T, k.shape[0], H,
+    check(lib().mc_prompt_attention(q.data_ptr(), qt, qh, k.data_ptr(), kt, kh,
+                                    v.data_ptr(), vt, vh, _ACT[q.dtype], T, k.shape[0], H,
                                     k.shape[1], D, _index(cu_q, "cu_q", dev),
                                     _index(cu_k, "cu_k", dev, (B + 1,)), B,
                                     D ** -0.5 if scale is None else scale, causal, out.data_ptr(),
