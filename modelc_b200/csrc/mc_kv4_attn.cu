@@ -106,21 +106,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // an 8x8 matrix o
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {  // two f32 fmas at once
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
-      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
-      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
 // The f16 pair (c - 8) of the codes in the low (ODD = 0) or second nibbles of
 // the halves of x.
 template <int ODD>

@@ -108,11 +108,6 @@ __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sy
 __device__ __forceinline__ void tm_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tm_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-__device__ __forceinline__ float ex2f(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -288,8 +283,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 
   // Of the block's 384 x 168 registers the softmax's two groups of warps take
   // 216 a thread and the third group keeps 72: 256 x 216 + 128 x 72 is the same.
-  if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-  else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   if (warp == 9) {
     // ----------------------------------------------------------- loads
     bool ok = true;
@@ -397,7 +392,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       }
       if (!ok && lane == 0) s_fail = 1;
     }
-  } else if (warp < 8) {
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // --------------------------------------------------------- softmax
     const int t = warp >> 2, row = t * kPromptRows + (warp & 3) * 32 + lane;
     const uint32_t base = tmem + ((uint32_t)(warp & 3) << 21);  // the warp's 32 lanes
@@ -420,14 +417,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
         for (int i = 0; i < 128; ++i) s[i] = i < left ? s[i] : 0xff800000u;
       }
-      float top = __uint_as_float(s[0]);
+      float top4[4];
 #pragma unroll
-      for (int i = 1; i < 128; ++i) top = fmaxf(top, __uint_as_float(s[i]));
+      for (int i = 0; i < 4; ++i) top4[i] = __uint_as_float(s[i]);
+#pragma unroll
+      for (int i = 4; i < 128; ++i) top4[i & 3] = fmaxf(top4[i & 3], __uint_as_float(s[i]));
+      const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
       const bool grown = (top - m) * c > kPromptGrow;  // also from -inf
       if (__any_sync(~0u, grown)) {
         const float mn = grown ? top : m;
         if (j > 0) {  // rescale O once the last product is in it
-          const float f = mn == m ? 1.f : m == -INFINITY ? 0.f : ex2f((m - mn) * c);
+          const float f = mn == m ? 1.f : m == -INFINITY ? 0.f : ex2((m - mn) * c);
           l *= f;
           ok = warp_wait(&b_pv[t], (j - 1) & 1);
           if (!ok) break;
@@ -445,20 +445,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         m = mn;
       }
       const float mc = m == -INFINITY ? 0.f : m * c;
-      float sum = 0.f;
+      float2 sum[2] = {};
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         uint32_t p[32];
 #pragma unroll
         for (int x = 0; x < 32; ++x) {
-          const float e0 = ex2f(fmaf(__uint_as_float(s[i * 64 + 2 * x]), c, -mc));
-          const float e1 = ex2f(fmaf(__uint_as_float(s[i * 64 + 2 * x + 1]), c, -mc));
-          sum += e0 + e1;
-          p[x] = pack2<T>(e0, e1);
+          float2 e = fma2(make_float2(__uint_as_float(s[i * 64 + 2 * x]), __uint_as_float(s[i * 64 + 2 * x + 1])),
+                          make_float2(c, c), make_float2(-mc, -mc));
+          e.x = ex2(e.x), e.y = ex2(e.y);
+          sum[x & 1] = add2(sum[x & 1], e);
+          p[x] = pack2<T>(e.x, e.y);
         }
         tm_store(ts + i * 32, p);
       }
-      l += sum;
+      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       tm_wait_st();
       tm_before();
       __syncwarp();
