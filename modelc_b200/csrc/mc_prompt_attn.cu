@@ -27,6 +27,7 @@ namespace mc {
 
 constexpr int kPromptRows = 128;  // rows of a query tile, keys of a key tile
 constexpr int kPromptThreads = 384;
+constexpr int kPromptPoly = 4;  // one pair of weights in so many by ex2_poly
 constexpr float kPromptGrow = 8.f;  // log2 growth of the maximum that is let pass
 
 struct PromptArgs {
@@ -108,6 +109,27 @@ __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sy
 __device__ __forceinline__ void tm_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tm_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+// 2^x on the f32 pipes, for part of a row: the special function unit's 16
+// exponentials a clock are as slow as the products they feed.  x = n + f with
+// |f| <= 1/2 by adding and taking away 1.5 * 2^23, whose last bits then hold
+// n; 2^f by the least-maximum-relative-error cubic (7.5e-5 = 2^-13.7, below
+// P's rounding); n goes into the exponent.  Below 2^-126 the result is 2^-126.
+// A NaN stays one through the clamp and leaves as a value beyond every type's
+// range, which the check of the results finds.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
+  const float2 big = make_float2(12582912.f, 12582912.f), one = make_float2(1.f, 1.f);
+  const float2 t = add2(x, big);
+  const float2 n = fma2(one, t, make_float2(-12582912.f, -12582912.f));
+  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+  float2 p = fma2(f, make_float2(0.05517167970538139f, 0.05517167970538139f),
+                  make_float2(0.24261116981506348f, 0.24261116981506348f));
+  p = fma2(p, f, make_float2(0.6932609677314758f, 0.6932609677314758f));
+  p = fma2(p, f, make_float2(0.9999280571937561f, 0.9999280571937561f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -231,7 +253,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (sm_ptr(smem_raw) & 1023u)) & 1023u);
   uint8_t *sq = smem, *ring = smem + 2 * C::Tile;
-  __shared__ __align__(8) uint64_t b_q, b_full[C::Slots], b_empty[C::Slots], b_s[2], b_p[2], b_pv[2], b_fix;
+  __shared__ __align__(8) uint64_t b_q[2], b_full[C::Slots], b_empty[C::Slots], b_s[2], b_p[2][2], b_pv[2],
+      b_tail, b_fix;
   __shared__ uint32_t s_tmem;
   __shared__ int s_fail;
   __shared__ PromptWork s_work;
@@ -248,10 +271,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   }
   if (warp == 0) prompt_work(a, index, &s_work);
   if (tid == 32) {
-    bar_init(&b_q, 1);
     for (int i = 0; i < C::Slots; ++i) bar_init(&b_full[i], 1), bar_init(&b_empty[i], 1);
-    for (int i = 0; i < 2; ++i) bar_init(&b_s[i], 1), bar_init(&b_p[i], 4), bar_init(&b_pv[i], 1);
-    bar_init(&b_fix, 1);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&b_q[i], 1), bar_init(&b_s[i], 1), bar_init(&b_pv[i], 1);
+      bar_init(&b_p[i][0], 4), bar_init(&b_p[i][1], 4);
+    }
+    bar_init(&b_tail, 1), bar_init(&b_fix, 1);
     s_fail = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -287,111 +312,116 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   if (warp == 9) {
     // ----------------------------------------------------------- loads
-    bool ok = true;
-    if (n_max > 0) {
-      if (lane == 0) {
-        const int tiles = n_t[1] ? 2 : 1;
-        bar_expect(&b_q, tiles * C::Tile);
-        for (int t = 0; t < tiles; ++t)
+    if (n_max > 0 && elect_one()) {
+      auto load_k = [&](int i) {  // K 0, V 0, K 1, V 1, ...
+        const int slot = i % C::Slots;
+        bar_expect(&b_full[slot], C::Tile);
+        for (int h = 0; h < NH; ++h)
+          load_tile(ring + slot * C::Tile + h * C::Half, i & 1 ? &mv : &mk, h * 64, hk, w.k0 + (i >> 1) * kPromptRows,
+                    &b_full[slot]);
+      };
+      for (int t = 0; t < 2; ++t) {
+        if (n_t[t]) {
+          bar_expect(&b_q[t], C::Tile);
           for (int h = 0; h < NH; ++h)
-            load_tile(sq + t * C::Tile + h * C::Half, &mq, h * 64, head, w.q0 + t * kPromptRows, &b_q);
-      }
-      for (int i = 0; i < 2 * n_max && ok; ++i) {  // K 0, V 0, K 1, V 1, ...
-        const int slot = i % C::Slots, use = i / C::Slots;
-        if (use) ok = warp_wait(&b_empty[slot], (use - 1) & 1);
-        if (lane == 0 && ok) {
-          bar_expect(&b_full[slot], C::Tile);
-          for (int h = 0; h < NH; ++h)
-            load_tile(ring + slot * C::Tile + h * C::Half, i & 1 ? &mv : &mk, h * 64, hk,
-                      w.k0 + (i >> 1) * kPromptRows, &b_full[slot]);
+            load_tile(sq + t * C::Tile + h * C::Half, &mq, h * 64, head, w.q0 + t * kPromptRows, &b_q[t]);
         }
-        __syncwarp();
+        if (t == 0) load_k(0);
       }
-      if (fix && ok) {
-        // the last V tile's rows behind the last key, as far as a product's
-        // 16 keys reach, become 0: what lies there is not this sequence's
-        const int i = 2 * n_max - 1, slot = i % C::Slots;
-        ok = warp_wait(&b_full[slot], (i / C::Slots) & 1);
-        if (ok)
-          for (int r = tail; r < (tail + 15) / 16 * 16; ++r)
-            for (int x = lane; x < NH * 8; x += 32)
-              *(uint4*)(ring + slot * C::Tile + (x / 8) * C::Half + r * 128 + (x % 8) * 16) = make_uint4(0, 0, 0, 0);
+      for (int i = 1; i < 2 * n_max; ++i) {
+        const int use = i / C::Slots;
+        if (use && !bar_wait(&b_empty[i % C::Slots], (use - 1) & 1)) {
+          s_fail = 1;
+          break;
+        }
+        load_k(i);
+      }
+    }
+  } else if (warp == 10) {
+    // The last V tile's rows behind the last key, as far as a product's 16
+    // keys reach, become 0: what lies there is not this sequence's.
+    if (fix) {
+      const int i = 2 * n_max - 1, slot = i % C::Slots;
+      // b_tail first: only then is the slot's last use the one whose parity is waited for
+      if (warp_wait(&b_tail, 0) && warp_wait(&b_full[slot], (i / C::Slots) & 1)) {
+        for (int r = tail; r < (tail + 15) / 16 * 16; ++r)
+          for (int x = lane; x < NH * 8; x += 32)
+            *(uint4*)(ring + slot * C::Tile + (x / 8) * C::Half + r * 128 + (x % 8) * 16) = make_uint4(0, 0, 0, 0);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) bar_arrive(&b_fix);
+      } else {
+        s_fail = 1;
       }
-      if (!ok && lane == 0) s_fail = 1;
     }
   } else if (warp == 8) {
     // -------------------------------------------------------- products
-    if (n_max > 0) {
-      bool ok = warp_wait(&b_q, 0);
+    if (n_max > 0 && elect_one()) {
       // f32 accumulator; type of A and B; B of P V has its columns contiguous; N; M
       constexpr uint32_t F = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
       const uint32_t id_s = (1u << 4) | (F << 7) | (F << 10) | ((a.scale < 0.f ? 1u : 0u) << 13) |
                             ((uint32_t)(kPromptRows >> 3) << 17) | ((uint32_t)(kPromptRows >> 4) << 24);
       const uint32_t id_o = (1u << 4) | (F << 7) | (F << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) |
                             ((uint32_t)(kPromptRows >> 4) << 24);
-      const bool one = elect_one();
       auto scores = [&](int t, int j) {
         const int slot = (2 * j) % C::Slots;
-        if (one) {
-          const uint64_t da = smem_desc(sm_ptr(sq + t * C::Tile), 16), db = smem_desc(sm_ptr(ring + slot * C::Tile), 16);
+        const uint64_t da = smem_desc(sm_ptr(sq + t * C::Tile), 16), db = smem_desc(sm_ptr(ring + slot * C::Tile), 16);
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint64_t off = (k % 4) * 2 + (k / 4) * (C::Half >> 4);
-            mma_ss(tmem + t * 128, da + off, db + off, id_s, k > 0);
-          }
-          mma_commit(&b_s[t]);
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t off = (k % 4) * 2 + (k / 4) * (C::Half >> 4);
+          mma_ss(tmem + t * 128, da + off, db + off, id_s, k > 0);
         }
-        __syncwarp();
+        mma_commit(&b_s[t]);
       };
-      auto values = [&](int t, int j) {
+      // half h of the tile's keys, 4 products of 16
+      auto values = [&](int t, int j, int h) {
         const int slot = (2 * j + 1) % C::Slots;
-        if (one) {
-          const uint64_t db = smem_desc(sm_ptr(ring + slot * C::Tile), C::Half);
-          const int steps = min(8, (lim[t] - j * kPromptRows + 15) / 16);
-          for (int k = 0; k < steps; ++k)
+        const uint64_t db = smem_desc(sm_ptr(ring + slot * C::Tile), C::Half);
+        const int steps = min(8, (lim[t] - j * kPromptRows + 15) / 16);
+#pragma unroll
+        for (int k = 4 * h; k < 4 * h + 4; ++k)
+          if (k < steps)
             mma_ts(tmem + C::O + t * D, tmem + t * 128 + k * 8, db + k * (2048 >> 4), id_o, j > 0 || k > 0);
-          mma_commit(&b_pv[t]);
-        }
-        __syncwarp();
       };
-      ok = ok && warp_wait(&b_full[0], 0);
-      if (ok) {
-        tm_after();
-        for (int t = 0; t < 2; ++t)
-          if (n_t[t]) scores(t, 0);
-        if (one) mma_commit(&b_empty[0]);
-      }
+      bool ok = bar_wait(&b_full[0], 0);
+      for (int t = 0; t < 2 && ok; ++t)
+        if (n_t[t]) {
+          ok = bar_wait(&b_q[t], 0);
+          tm_after();
+          if (ok) scores(t, 0);
+        }
+      if (ok) mma_commit(&b_empty[0]);
       for (int j = 0; j < n_max && ok; ++j) {
         const int vi = 2 * j + 1, ki = 2 * j + 2;
-        bool have_k = false;
-        ok = warp_wait(&b_full[vi % C::Slots], (vi / C::Slots) & 1);
-        if (j == n_max - 1 && fix) ok = ok && warp_wait(&b_fix, 0);
+        const bool more = j + 1 < n_max;
+        ok = bar_wait(&b_full[vi % C::Slots], (vi / C::Slots) & 1);
+        if (!more && fix && ok) {
+          bar_arrive(&b_tail);
+          ok = bar_wait(&b_fix, 0);
+        }
+        if (more) ok = ok && bar_wait(&b_full[ki % C::Slots], (ki / C::Slots) & 1);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (j >= n_t[t]) continue;
-          ok = ok && warp_wait(&b_p[t], j & 1);
+          ok = ok && bar_wait(&b_p[t][0], j & 1);
           if (!ok) break;
           tm_after();
-          values(t, j);
-          if (j + 1 < n_t[t]) {
-            if (!have_k) {
-              ok = warp_wait(&b_full[ki % C::Slots], (ki / C::Slots) & 1);
-              have_k = true;
-            }
-            if (ok) scores(t, j + 1);
-          }
+          values(t, j, 0);
+          ok = bar_wait(&b_p[t][1], j & 1);
+          if (!ok) break;
+          tm_after();
+          values(t, j, 1);
+          mma_commit(&b_pv[t]);
+          if (j + 1 < n_t[t]) scores(t, j + 1);
         }
-        if (ok && one) {
+        if (ok) {
           mma_commit(&b_empty[vi % C::Slots]);
-          if (have_k) mma_commit(&b_empty[ki % C::Slots]);
+          if (more) mma_commit(&b_empty[ki % C::Slots]);
         }
-        __syncwarp();
       }
-      if (!ok && lane == 0) s_fail = 1;
+      if (!ok) s_fail = 1;
     }
+    __syncwarp();
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -400,7 +430,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     const uint32_t base = tmem + ((uint32_t)(warp & 3) << 21);  // the warp's 32 lanes
     const uint32_t ts = base + t * 128, to = base + C::O + t * D;
     const int n = n_t[t];
-    const int see = row < w.n_q ? min(max(row + w.shift, 0), w.L) : 0;  // keys of this row
+    // keys of this row; rows past the sequence go with its last one
+    const int see = min(max(min(row, w.n_q - 1) + w.shift, 0), w.L);
     const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
@@ -413,7 +444,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       for (int i = 0; i < 4; ++i) tm_load(ts + i * 32, s + i * 32);
       tm_wait_ld();
       const int left = see - j * kPromptRows;  // visible columns
-      if (!__all_sync(~0u, left >= kPromptRows)) {
+      const bool all = __all_sync(~0u, left >= kPromptRows);
+      if (!all) {
 #pragma unroll
         for (int i = 0; i < 128; ++i) s[i] = i < left ? s[i] : 0xff800000u;
       }
@@ -446,24 +478,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       }
       const float mc = m == -INFINITY ? 0.f : m * c;
       float2 sum[2] = {};
+      auto weights = [&](auto mask) {
+        constexpr bool MASK = decltype(mask)::value;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t p[32];
+        for (int i = 0; i < 2; ++i) {
+          uint32_t p[32];
 #pragma unroll
-        for (int x = 0; x < 32; ++x) {
-          float2 e = fma2(make_float2(__uint_as_float(s[i * 64 + 2 * x]), __uint_as_float(s[i * 64 + 2 * x + 1])),
-                          make_float2(c, c), make_float2(-mc, -mc));
-          e.x = ex2(e.x), e.y = ex2(e.y);
-          sum[x & 1] = add2(sum[x & 1], e);
-          p[x] = pack2<T>(e.x, e.y);
+          for (int x = 0; x < 32; ++x) {
+            float2 e = fma2(make_float2(__uint_as_float(s[i * 64 + 2 * x]), __uint_as_float(s[i * 64 + 2 * x + 1])),
+                            make_float2(c, c), make_float2(-mc, -mc));
+            if (!MASK && x % kPromptPoly == kPromptPoly - 1) e = ex2_poly(e);
+            else e.x = ex2(e.x), e.y = ex2(e.y);
+            sum[x & 1] = add2(sum[x & 1], e);
+            p[x] = pack2<T>(e.x, e.y);
+          }
+          tm_store(ts + i * 32, p);
+          tm_wait_st();
+          tm_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(&b_p[t][i]);
         }
-        tm_store(ts + i * 32, p);
-      }
+      };
+      if (all) weights(std::false_type());
+      else weights(std::true_type());
       l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-      tm_wait_st();
-      tm_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(&b_p[t]);
     }
     // ------------------------------------------------------- the result
     if (n > 0) ok = ok && warp_wait(&b_pv[t], (n - 1) & 1);
@@ -471,9 +509,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     tm_after();
     const float f = l != 0.f ? 1.f / l : 0.f;
     const bool live = row < w.n_q;
-    T* out = (T*)a.out + ((size_t)(w.q0 + row) * a.H + head) * D;
     bool bad = false;
     if (n > 0 && ok) {
+      // the warp's rows go through its part of the tile's queries, which the
+      // products no longer read, so that whole rows are written at once
+      uint8_t* stage = sq + t * C::Tile + (warp & 3) * 32 * D * 2;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
         uint32_t o[32], y[16];
@@ -481,17 +521,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         tm_wait_ld();
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
-          // a row without keys has l = 0 and P = 0: its O may still hold NaN
           const float y0 = __uint_as_float(o[2 * x]) * f, y1 = __uint_as_float(o[2 * x + 1]) * f;
           bad |= !(fabsf(y0) <= 3e38f) || !(fabsf(y1) <= 3e38f);
           y[x] = pack2<T>(y0, y1);
         }
-        if (live)
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            *(uint4*)(out + i * 32 + x * 8) = make_uint4(y[4 * x], y[4 * x + 1], y[4 * x + 2], y[4 * x + 3]);
+        for (int x = 0; x < 4; ++x)
+          *(uint4*)(stage + lane * D * 2 + (((i * 4 + x) ^ lane) % (D / 8)) * 16) =
+              make_uint4(y[4 * x], y[4 * x + 1], y[4 * x + 2], y[4 * x + 3]);
+      }
+      __syncwarp();
+      const int first = t * kPromptRows + (warp & 3) * 32;
+#pragma unroll 4
+      for (int i = lane; i < 32 * (D / 8); i += 32) {
+        const int r = i / (D / 8), x = i % (D / 8);
+        if (first + r < w.n_q)
+          *(uint4*)((T*)a.out + ((size_t)(w.q0 + first + r) * a.H + head) * D + x * 8) =
+              *(const uint4*)(stage + r * D * 2 + ((x ^ r) % (D / 8)) * 16);
       }
     } else if (live) {  // no keys; or a wait ran out
+      T* out = (T*)a.out + ((size_t)(w.q0 + row) * a.H + head) * D;
       const uint32_t y = ok ? 0u : 0x7fff7fffu;
       for (int x = 0; x < D / 8; ++x) *(uint4*)(out + x * 8) = make_uint4(y, y, y, y);
     }
@@ -503,8 +552,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     tm_before();
   }
   __syncthreads();
-  if (s_fail && warp == 9 ) {  // leave no copy in flight
-    warp_wait(&b_q, 0);
+  if (s_fail && warp == 9) {  // leave no copy in flight
+    for (int t = 0; t < 2; ++t)
+      if (n_t[t]) warp_wait(&b_q[t], 0);
     for (int i = max(0, 2 * n_max - C::Slots); i < 2 * n_max; ++i) warp_wait(&b_full[i % C::Slots], (i / C::Slots) & 1);
   }
   if (warp == 8) {
