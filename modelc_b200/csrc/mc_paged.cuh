@@ -137,18 +137,26 @@ __device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
 }
 // Waits for the phase with this parity, two seconds at most: far above any
 // copy's or product's time, so it runs out only when something else failed.
-__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity) {
-  for (int i = 0; i < 64; ++i)
-    if (bar_try(b, parity)) return true;
-  unsigned long long t0, t1;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-  do {
-    for (int i = 0; i < 64; ++i)
-      if (bar_try(b, parity)) return true;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1));
-  } while (t1 - t0 < 2000000000ull);
-  return false;
+__device__ __forceinline__ bool bar_loop(uint32_t b, uint32_t parity) {
+  unsigned long long t0 = 0, t1;
+  for (int i = 0;; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(b), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if (i % 64 == 63) {
+      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1));
+      if (!t0) t0 = t1;
+      if (t1 - t0 > 2000000000ull) return false;
+    }
+  }
 }
+__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity) { return bar_loop(sm_ptr(b), parity); }
 // The same for a whole warp: true where no lane's wait ran out.
 __device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity) {
   return __all_sync(~0u, bar_wait(b, parity));

@@ -27,7 +27,11 @@ namespace mc {
 
 constexpr int kPromptRows = 128;  // rows of a query tile, keys of a key tile
 constexpr int kPromptThreads = 384;
-constexpr int kPromptPoly = 4;  // one pair of weights in so many by ex2_poly
+// Barriers of the rounds of products: round 0 is the first scores, round j + 1
+// the values j and the scores j + 1.  The loads run at most Slots / 2 rounds
+// ahead of the round that they wait for, so with more barriers than that no
+// barrier is two phases ahead of a waiting load.
+constexpr int kPromptRounds = 8;
 constexpr float kPromptGrow = 8.f;  // log2 growth of the maximum that is let pass
 
 struct PromptArgs {
@@ -63,29 +67,38 @@ __device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* m, int x
       "l"(m), "r"(x), "r"(h), "r"(t), "r"(sm_ptr(b))
       : "memory");
 }
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo) {
-  // start, leading and stride byte offsets in 16-byte units (8 rows of 128
-  // bytes are 1024), descriptor version 1, 128-byte swizzle
-  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         (1ull << 46) | (2ull << 61);
+// Shared-memory descriptors: the low word has the start address and the
+// leading byte offset, the high word the stride (8 rows of 128 bytes), the
+// version 1 and the 128-byte swizzle; offsets count 16 bytes.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) {
+  return ((addr >> 4) & 0x3FFF) | ((lbo >> 4) << 16);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
+// The products are issued by the lane whose `one` is set.  All lanes run the
+// code around them, so that its values stay in uniform registers: with one
+// lane inside a branch each product waited for its operands to be moved there.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc, uint32_t one) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "mov.b64 a, {%1, %6};\n\tmov.b64 b, {%2, %6};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(one), "r"(kDescHi)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc, uint32_t one) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "mov.b64 b, {%2, %6};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(one), "r"(kDescHi)
       : "memory");
 }
-__device__ __forceinline__ void mma_commit(uint64_t* b) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(sm_ptr(b))
-               : "memory");
+__device__ __forceinline__ void mma_commit(uint64_t* b, uint32_t one) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(sm_ptr(b)),
+      "r"(one)
+      : "memory");
 }
 #define MC_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
 #define MC_I8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
@@ -109,27 +122,6 @@ __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sy
 __device__ __forceinline__ void tm_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tm_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// 2^x on the f32 pipes, for part of a row: the special function unit's 16
-// exponentials a clock are as slow as the products they feed.  x = n + f with
-// |f| <= 1/2 by adding and taking away 1.5 * 2^23, whose last bits then hold
-// n; 2^f by the least-maximum-relative-error cubic (7.5e-5 = 2^-13.7, below
-// P's rounding); n goes into the exponent.  Below 2^-126 the result is 2^-126.
-// A NaN stays one through the clamp and leaves as a value beyond every type's
-// range, which the check of the results finds.
-__device__ __forceinline__ float2 ex2_poly(float2 x) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
-  const float2 big = make_float2(12582912.f, 12582912.f), one = make_float2(1.f, 1.f);
-  const float2 t = add2(x, big);
-  const float2 n = fma2(one, t, make_float2(-12582912.f, -12582912.f));
-  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
-  float2 p = fma2(f, make_float2(0.05517167970538139f, 0.05517167970538139f),
-                  make_float2(0.24261116981506348f, 0.24261116981506348f));
-  p = fma2(p, f, make_float2(0.6932609677314758f, 0.6932609677314758f));
-  p = fma2(p, f, make_float2(0.9999280571937561f, 0.9999280571937561f));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
-}
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -145,6 +137,13 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
   uint32_t x;
   memcpy(&x, &h, 4);
   return x;
+}
+
+// One copy of the polling loop for the waits of the loading and the issuing
+// thread, so that the code between them is short.
+__device__ __noinline__ bool bar_poll(uint32_t b, uint32_t parity) { return bar_loop(b, parity); }
+__device__ __forceinline__ bool bar_wait_far(uint64_t* b, uint32_t parity) {
+  return bar_try(b, parity) || bar_poll(sm_ptr(b), parity);
 }
 
 struct PromptWork {
@@ -253,7 +252,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (sm_ptr(smem_raw) & 1023u)) & 1023u);
   uint8_t *sq = smem, *ring = smem + 2 * C::Tile;
-  __shared__ __align__(8) uint64_t b_q[2], b_full[C::Slots], b_empty[C::Slots], b_s[2], b_p[2][2], b_pv[2],
+  __shared__ __align__(8) uint64_t b_q[2], b_full[C::Slots], b_round[kPromptRounds], b_s[2], b_p[2][2], b_pv[2],
       b_tail, b_fix;
   __shared__ uint32_t s_tmem;
   __shared__ int s_fail;
@@ -271,7 +270,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   }
   if (warp == 0) prompt_work(a, index, &s_work);
   if (tid == 32) {
-    for (int i = 0; i < C::Slots; ++i) bar_init(&b_full[i], 1), bar_init(&b_empty[i], 1);
+    for (int i = 0; i < C::Slots; ++i) bar_init(&b_full[i], 1);
+    for (int i = 0; i < kPromptRounds; ++i) bar_init(&b_round[i], 1);
     for (int i = 0; i < 2; ++i) {
       bar_init(&b_q[i], 1), bar_init(&b_s[i], 1), bar_init(&b_pv[i], 1);
       bar_init(&b_p[i][0], 4), bar_init(&b_p[i][1], 4);
@@ -329,8 +329,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (t == 0) load_k(0);
       }
       for (int i = 1; i < 2 * n_max; ++i) {
-        const int use = i / C::Slots;
-        if (use && !bar_wait(&b_empty[i % C::Slots], (use - 1) & 1)) {
+        // the slot's last tile was number i - Slots: K j is read in round j, V j in round j + 1
+        const int last = i - C::Slots, round = (last + 1) >> 1;
+        if (last >= 0 && !bar_wait_far(&b_round[round % kPromptRounds], (round / kPromptRounds) & 1)) {
           s_fail = 1;
           break;
         }
@@ -356,70 +357,68 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
   } else if (warp == 8) {
     // -------------------------------------------------------- products
-    if (n_max > 0 && elect_one()) {
+    if (n_max > 0) {
       // f32 accumulator; type of A and B; B of P V has its columns contiguous; N; M
       constexpr uint32_t F = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
       const uint32_t id_s = (1u << 4) | (F << 7) | (F << 10) | ((a.scale < 0.f ? 1u : 0u) << 13) |
                             ((uint32_t)(kPromptRows >> 3) << 17) | ((uint32_t)(kPromptRows >> 4) << 24);
       const uint32_t id_o = (1u << 4) | (F << 7) | (F << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) |
                             ((uint32_t)(kPromptRows >> 4) << 24);
-      auto scores = [&](int t, int j) {
-        const int slot = (2 * j) % C::Slots;
-        const uint64_t da = smem_desc(sm_ptr(sq + t * C::Tile), 16), db = smem_desc(sm_ptr(ring + slot * C::Tile), 16);
+      const uint32_t one = elect_one();
+      const uint32_t d_q = desc_lo(sm_ptr(sq), 16), d_k = desc_lo(sm_ptr(ring), 16), d_v = desc_lo(sm_ptr(ring), C::Half);
+      auto scores = [&](int t, int slot) {
+        const uint32_t da = d_q + t * (C::Tile >> 4), db = d_k + slot * (C::Tile >> 4);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint64_t off = (k % 4) * 2 + (k / 4) * (C::Half >> 4);
-          mma_ss(tmem + t * 128, da + off, db + off, id_s, k > 0);
+          const uint32_t off = (k % 4) * 2 + (k / 4) * (C::Half >> 4);
+          mma_ss(tmem + t * 128, da + off, db + off, id_s, k > 0, one);
         }
-        mma_commit(&b_s[t]);
-      };
-      // half h of the tile's keys, 4 products of 16
-      auto values = [&](int t, int j, int h) {
-        const int slot = (2 * j + 1) % C::Slots;
-        const uint64_t db = smem_desc(sm_ptr(ring + slot * C::Tile), C::Half);
-        const int steps = min(8, (lim[t] - j * kPromptRows + 15) / 16);
-#pragma unroll
-        for (int k = 4 * h; k < 4 * h + 4; ++k)
-          if (k < steps)
-            mma_ts(tmem + C::O + t * D, tmem + t * 128 + k * 8, db + k * (2048 >> 4), id_o, j > 0 || k > 0);
+        mma_commit(&b_s[t], one);
       };
       bool ok = bar_wait(&b_full[0], 0);
-      for (int t = 0; t < 2 && ok; ++t)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
         if (n_t[t]) {
-          ok = bar_wait(&b_q[t], 0);
+          ok &= bar_wait(&b_q[t], 0);
           tm_after();
-          if (ok) scores(t, 0);
+          scores(t, 0);
         }
-      if (ok) mma_commit(&b_empty[0]);
+      mma_commit(&b_round[0], one);
+      int vs = 1, ks = 2, vp = 0, kp = 0;  // slots of V j and K j + 1, their parities
+#pragma unroll 1
       for (int j = 0; j < n_max && ok; ++j) {
-        const int vi = 2 * j + 1, ki = 2 * j + 2;
         const bool more = j + 1 < n_max;
-        ok = bar_wait(&b_full[vi % C::Slots], (vi / C::Slots) & 1);
-        if (!more && fix && ok) {
-          bar_arrive(&b_tail);
-          ok = bar_wait(&b_fix, 0);
+        ok = bar_wait(&b_full[vs], vp);
+        if (more) ok &= bar_wait(&b_full[ks], kp);
+        if (!more && fix) {
+          if (one) bar_arrive(&b_tail);
+          __syncwarp();
+          ok &= bar_wait(&b_fix, 0);
         }
-        if (more) ok = ok && bar_wait(&b_full[ki % C::Slots], (ki / C::Slots) & 1);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (j >= n_t[t]) continue;
-          ok = ok && bar_wait(&b_p[t][0], j & 1);
-          if (!ok) break;
-          tm_after();
-          values(t, j, 0);
-          ok = bar_wait(&b_p[t][1], j & 1);
-          if (!ok) break;
-          tm_after();
-          values(t, j, 1);
-          mma_commit(&b_pv[t]);
-          if (j + 1 < n_t[t]) scores(t, j + 1);
+          const int steps = min(8, (lim[t] - j * kPromptRows + 15) / 16);
+          const uint32_t db = d_v + vs * (C::Tile >> 4);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // the halves of P
+            ok &= bar_wait(&b_p[t][h], j & 1);
+            tm_after();
+#pragma unroll
+            for (int k = 4 * h; k < 4 * h + 4; ++k)
+              mma_ts(tmem + C::O + t * D, tmem + t * 128 + k * 8, db + k * (2048 >> 4), id_o, j > 0 || k > 0,
+                     k < steps ? one : 0);
+          }
+          // the scores' commit stands for the values before them too
+          if (j + 1 < n_t[t]) scores(t, ks);
+          else mma_commit(&b_pv[t], one);
         }
-        if (ok) {
-          mma_commit(&b_empty[vi % C::Slots]);
-          if (more) mma_commit(&b_empty[ki % C::Slots]);
-        }
+        if (more) mma_commit(&b_round[(j + 1) % kPromptRounds], one);
+        if ((vs += 2) >= C::Slots) vs -= C::Slots, vp ^= 1;
+        if ((ks += 2) >= C::Slots) ks -= C::Slots, kp ^= 1;
+        ok = __all_sync(~0u, ok);
       }
-      if (!ok) s_fail = 1;
+      if (!ok && one) s_fail = 1;
     }
     __syncwarp();
   }
@@ -444,8 +443,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       for (int i = 0; i < 4; ++i) tm_load(ts + i * 32, s + i * 32);
       tm_wait_ld();
       const int left = see - j * kPromptRows;  // visible columns
-      const bool all = __all_sync(~0u, left >= kPromptRows);
-      if (!all) {
+      if (!__all_sync(~0u, left >= kPromptRows)) {
 #pragma unroll
         for (int i = 0; i < 128; ++i) s[i] = i < left ? s[i] : 0xff800000u;
       }
@@ -458,12 +456,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const bool grown = (top - m) * c > kPromptGrow;  // also from -inf
       if (__any_sync(~0u, grown)) {
         const float mn = grown ? top : m;
-        if (j > 0) {  // rescale O once the last product is in it
+        if (j > 0) {  // rescale O: the products before these scores are in it
           const float f = mn == m ? 1.f : m == -INFINITY ? 0.f : ex2((m - mn) * c);
           l *= f;
-          ok = warp_wait(&b_pv[t], (j - 1) & 1);
-          if (!ok) break;
-          tm_after();
 #pragma unroll
           for (int i = 0; i < D / 32; ++i) {
             uint32_t o[32];
@@ -478,33 +473,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       }
       const float mc = m == -INFINITY ? 0.f : m * c;
       float2 sum[2] = {};
-      auto weights = [&](auto mask) {
-        constexpr bool MASK = decltype(mask)::value;
+      // (a cubic on the f32 pipes for a part of the exponentials was measured
+      // slower, 936 against 977 TFLOP/s: the special function unit is not
+      // what a tile waits for)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t p[32];
+      for (int i = 0; i < 2; ++i) {
+        uint32_t p[32];
 #pragma unroll
-          for (int x = 0; x < 32; ++x) {
-            float2 e = fma2(make_float2(__uint_as_float(s[i * 64 + 2 * x]), __uint_as_float(s[i * 64 + 2 * x + 1])),
-                            make_float2(c, c), make_float2(-mc, -mc));
-            if (!MASK && x % kPromptPoly == kPromptPoly - 1) e = ex2_poly(e);
-            else e.x = ex2(e.x), e.y = ex2(e.y);
-            sum[x & 1] = add2(sum[x & 1], e);
-            p[x] = pack2<T>(e.x, e.y);
-          }
-          tm_store(ts + i * 32, p);
-          tm_wait_st();
-          tm_before();
-          __syncwarp();
-          if (lane == 0) bar_arrive(&b_p[t][i]);
+        for (int x = 0; x < 32; ++x) {
+          float2 e = fma2(make_float2(__uint_as_float(s[i * 64 + 2 * x]), __uint_as_float(s[i * 64 + 2 * x + 1])),
+                          make_float2(c, c), make_float2(-mc, -mc));
+          e.x = ex2(e.x), e.y = ex2(e.y);
+          sum[x & 1] = add2(sum[x & 1], e);
+          p[x] = pack2<T>(e.x, e.y);
         }
-      };
-      if (all) weights(std::false_type());
-      else weights(std::true_type());
+        tm_store(ts + i * 32, p);
+        tm_wait_st();
+        tm_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&b_p[t][i]);
+      }
       l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
     }
     // ------------------------------------------------------- the result
-    if (n > 0) ok = ok && warp_wait(&b_pv[t], (n - 1) & 1);
+    if (n > 0) ok = ok && warp_wait(&b_pv[t], 0);
     if (!ok) s_fail = 1;
     tm_after();
     const float f = l != 0.f ? 1.f / l : 0.f;
