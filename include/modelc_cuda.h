@@ -447,12 +447,14 @@ MC_API mc_status mc_sample_rows(const float* logits_dev, int32_t n_rows, int32_t
  * -1, as tokens beyond table_width pages get slot -1.  n_tokens must be at
  * least the sum of q_len: tokens beyond it are not placed.  Inputs other than
  * the table are left as they are, so a step can be planned again. */
-MC_API mc_status mc_paged_slots(const int32_t* kv_len, const int32_t* q_len, int32_t n_requests,
-                                int32_t* table, int32_t table_width, const int32_t* free_pages,
-                                int32_t n_free_pages, const int32_t* n_free, int32_t page_size,
-                                int32_t n_tokens, int32_t* cu_q, int32_t* positions,
-                                int32_t* slots, int32_t* new_len, int32_t* n_free_out,
-                                int32_t device, void* stream);
+typedef struct mc_slots_args {
+  const int32_t *kv_len, *q_len;
+  int32_t* table;
+  const int32_t *free_pages, *n_free;
+  int32_t *cu_q, *positions, *slots, *new_len, *n_free_out;
+  int32_t n_requests, table_width, n_free_pages, page_size, n_tokens;
+} mc_slots_args;
+MC_API mc_status mc_paged_slots(const mc_slots_args* args, int32_t device, void* stream);
 
 /* Tables [positions][n_freq] of factor * cos and sin of position * freq, in
  * f64, rounded once to f32 (freq: device memory). */
@@ -468,12 +470,15 @@ MC_API mc_status mc_rope_table(const double* freq, int32_t n_freq, int32_t posit
  * the inputs' type, or for f32 inputs of any; an output may be its own
  * contiguous input when the types agree.  A position outside the tables gives
  * NaN. */
-MC_API mc_status mc_rope(const void* q, int64_t q_tok, int64_t q_head, int32_t n_heads,
-                         const void* k, int64_t k_tok, int64_t k_head, int32_t n_kv_heads,
-                         int32_t dtype, int32_t n_tokens, int32_t head_dim, int32_t rot,
-                         int32_t interleaved, const int32_t* positions, const float* cos_table,
-                         const float* sin_table, int32_t table_rows, void* q_out, void* k_out,
-                         int32_t out_dtype, int32_t device, void* stream);
+typedef struct mc_rope_args {
+  const void *q, *k;
+  const int32_t* positions;
+  const float *cos_table, *sin_table;
+  void *q_out, *k_out;
+  int64_t q_tok, q_head, k_tok, k_head; /* strides of the inputs */
+  int32_t n_heads, n_kv_heads, dtype, out_dtype, n_tokens, head_dim, rot, interleaved, table_rows;
+} mc_rope_args;
+MC_API mc_status mc_rope(const mc_rope_args* args, int32_t device, void* stream);
 
 /* The 4-bit cache is a pool of pages [n_pages][n_kv_heads] of
  * mc_kv4_page_bytes(head_dim) bytes each (0 for an unsupported head dim; 64
@@ -485,47 +490,60 @@ MC_API mc_status mc_rope(const void* q, int64_t q_tok, int64_t q_head, int32_t n
 MC_API int64_t mc_kv4_page_bytes(int32_t head_dim);
 /* k, v [n_tokens][n_kv_heads][head_dim] into their slots; slots outside the
  * pool are skipped.  No two tokens of one call may share a slot. */
-MC_API mc_status mc_kv4_append(void* pool, int64_t n_pages, int32_t n_kv_heads, int32_t head_dim,
-                               const void* k, int64_t k_tok, int64_t k_head, const void* v,
-                               int64_t v_tok, int64_t v_head, int32_t dtype,
-                               const int32_t* slots, int32_t n_tokens, int32_t device,
-                               void* stream);
+typedef struct mc_kv4_append_args {
+  void* pool;
+  const void *k, *v;
+  const int32_t* slots;
+  int64_t n_pages, k_tok, k_head, v_tok, v_head;
+  int32_t n_kv_heads, head_dim, dtype, n_tokens;
+} mc_kv4_append_args;
+MC_API mc_status mc_kv4_append(const mc_kv4_append_args* args, int32_t device, void* stream);
 /* The values of n_tokens slots, contiguous; slots outside the pool read as 0. */
-MC_API mc_status mc_kv4_read(const void* pool, int64_t n_pages, int32_t n_kv_heads,
-                             int32_t head_dim, const int32_t* slots, int32_t n_tokens, void* k_out,
-                             void* v_out, int32_t dtype, int32_t device, void* stream);
+typedef struct mc_kv4_read_args {
+  const void* pool;
+  const int32_t* slots;
+  void *k_out, *v_out;
+  int64_t n_pages;
+  int32_t n_kv_heads, head_dim, dtype, n_tokens;
+} mc_kv4_read_args;
+MC_API mc_status mc_kv4_read(const mc_kv4_read_args* args, int32_t device, void* stream);
 
 /* Attention of the new tokens of n_requests requests over the 4-bit cache:
  * softmax(scale q k^T) v, query head h reading key/value head h / (n_heads /
  * n_kv_heads).  Rows cu_q[z] .. cu_q[z + 1] of q belong to request z and are
  * the last of its kv_len[z] tokens (the cache holds them already): row j sees
  * the tokens up to its own.  A row that sees none, and a row of no request,
- * gives 0; so does a page whose table entry lies outside the pool count as
- * not there.  q and out are f16 or bf16; out is contiguous.  The workspace
+ * gives 0; a page whose table entry lies outside the pool counts as not
+ * there.  q and out are f16 or bf16; out is contiguous.  The workspace
  * (16-byte aligned, of the size that mc_kv4_attention_workspace gives, 0 on
  * an error) needs no clearing and is free again when the call has run. */
+typedef struct mc_kv4_attention_args {
+  const void *q, *pool;
+  const int32_t *table, *kv_len, *cu_q;
+  void *out, *workspace;
+  int64_t q_tok, q_head, n_pages, workspace_bytes;
+  int32_t dtype, n_tokens, n_heads, n_kv_heads, head_dim, table_width, n_requests;
+  float scale;
+} mc_kv4_attention_args;
 MC_API int64_t mc_kv4_attention_workspace(int32_t n_requests, int32_t head_dim, int32_t device);
-MC_API mc_status mc_kv4_attention(const void* q, int64_t q_tok, int64_t q_head, int32_t dtype,
-                                  int32_t n_tokens, int32_t n_heads, const void* pool,
-                                  int64_t n_pages, int32_t n_kv_heads, int32_t head_dim,
-                                  const int32_t* table, int32_t table_width,
-                                  const int32_t* kv_len, const int32_t* cu_q,
-                                  int32_t n_requests, float scale, void* out, void* workspace,
-                                  int64_t workspace_bytes, int32_t device, void* stream);
+MC_API mc_status mc_kv4_attention(const mc_kv4_attention_args* args, int32_t device, void* stream);
 
 /* Attention over packed prompts: sequence z has queries cu_q[z] .. cu_q[z +
  * 1] of q [n_q][n_heads][head_dim] and keys cu_k[z] .. cu_k[z + 1] of k and v
- * [n_k][n_kv_heads][head_dim] (f16 or bf16, all of one type).  Causal: the
- * sequence's queries are its last tokens, so query i sees the keys up to i +
- * (keys - queries).  A row that sees no key, and a row of no sequence, gives
- * 0.  out is contiguous, of q's type. */
-MC_API mc_status mc_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void* k,
-                                     int64_t k_tok, int64_t k_head, const void* v, int64_t v_tok,
-                                     int64_t v_head, int32_t dtype, int32_t n_q, int32_t n_k,
-                                     int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
-                                     const int32_t* cu_q, const int32_t* cu_k,
-                                     int32_t n_sequences, float scale, int32_t causal, void* out,
-                                     int32_t device, void* stream);
+ * [n_k][n_kv_heads][head_dim] (f16 or bf16, all of one type, every head's row
+ * at a multiple of 16 bytes).  Causal: the sequence's queries are its last
+ * tokens, so query i sees the keys up to i + (keys - queries).  A row that
+ * sees no key, and a row of no sequence, gives 0.  out is contiguous, of q's
+ * type. */
+typedef struct mc_prompt_args {
+  const void *q, *k, *v;
+  const int32_t *cu_q, *cu_k;
+  void* out;
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
+  int32_t dtype, n_q, n_k, n_heads, n_kv_heads, head_dim, n_sequences, causal;
+  float scale;
+} mc_prompt_args;
+MC_API mc_status mc_prompt_attention(const mc_prompt_args* args, int32_t device, void* stream);
 
 MC_API size_t mc_last_error(char* buf, size_t cap);
 MC_API const char* mc_version(void);

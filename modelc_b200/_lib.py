@@ -145,20 +145,16 @@ def lib():
         "mc_ngram_draft_destroy": (i32, [vp]),
         "mc_sample_rows": (i32, [vp, i32, i32, C.c_float, C.c_float, C.c_float, C.c_uint64,
                                  C.c_uint32, vp, vp]),
-        "mc_paged_slots": (i32, [vp, vp, i32, vp, i32, vp, i32, vp, i32, i32, vp, vp, vp, vp, vp,
-                                 i32, vp]),
+        # the argument structs of these are packed by paged.py
+        "mc_paged_slots": (i32, [C.c_char_p, i32, vp]),
         "mc_rope_table": (i32, [vp, i32, i32, C.c_double, vp, vp, i32, vp]),
-        "mc_rope": (i32, [vp, i64, i64, i32, vp, i64, i64, i32, i32, i32, i32, i32, i32, vp, vp,
-                          vp, i32, vp, vp, i32, i32, vp]),
+        "mc_rope": (i32, [C.c_char_p, i32, vp]),
         "mc_kv4_page_bytes": (i64, [i32]),
-        "mc_kv4_append": (i32, [vp, i64, i32, i32, vp, i64, i64, vp, i64, i64, i32, vp, i32, i32,
-                                vp]),
-        "mc_kv4_read": (i32, [vp, i64, i32, i32, vp, i32, vp, vp, i32, i32, vp]),
-        "mc_kv4_attention": (i32, [vp, i64, i64, i32, i32, i32, vp, i64, i32, i32, vp, i32, vp,
-                                   vp, i32, C.c_float, vp, vp, i64, i32, vp]),
+        "mc_kv4_append": (i32, [C.c_char_p, i32, vp]),
+        "mc_kv4_read": (i32, [C.c_char_p, i32, vp]),
         "mc_kv4_attention_workspace": (i64, [i32, i32, i32]),
-        "mc_prompt_attention": (i32, [vp, i64, i64, vp, i64, i64, vp, i64, i64, i32, i32, i32, i32,
-                                      i32, i32, vp, vp, i32, C.c_float, i32, vp, i32, vp]),
+        "mc_kv4_attention": (i32, [C.c_char_p, i32, vp]),
+        "mc_prompt_attention": (i32, [C.c_char_p, i32, vp]),
         "mc_session_stream": (vp, [vp]),
         "mc_session_round_launches": (i32, [vp]),
         "mc_version": (C.c_char_p, []),

@@ -68,8 +68,8 @@ __device__ __forceinline__ Kv4Req kv4_req(const Kv4Args& a, int z) {
   Kv4Req r;
   r.c0 = min(max(__ldg(a.cu_q + z), 0), a.T);
   r.n = max(min(__ldg(a.cu_q + z + 1), a.T) - r.c0, 0);
-  r.kv = max(__ldg(a.kv_len + z), 0);
-  r.nb = (r.n * (a.H / a.Hk) + R - 1) / R;
+  r.kv = min(max(__ldg(a.kv_len + z), 0), 0x7fffff00);
+  r.nb = (int)(((long long)r.n * (a.H / a.Hk) + R - 1) / R);
   // a request without tokens has one page that counts as absent
   r.pages = r.n ? max(1, min((r.kv + kKv4Page - 1) / kKv4Page, a.width)) : 0;
   return r;
@@ -741,13 +741,17 @@ extern "C" int64_t mc_kv4_attention_workspace(int32_t n_requests, int32_t head_d
                            kv4_space(sms, n_requests, 24, head_dim).total);
 }
 
-extern "C" mc_status mc_kv4_attention(const void* q, int64_t q_tok, int64_t q_head, int32_t dtype,
-                                      int32_t n_tokens, int32_t n_heads, const void* pool,
-                                      int64_t n_pages, int32_t n_kv_heads, int32_t head_dim,
-                                      const int32_t* table, int32_t table_width,
-                                      const int32_t* kv_len, const int32_t* cu_q,
-                                      int32_t n_requests, float scale, void* out, void* workspace,
-                                      int64_t workspace_bytes, int32_t device, void* stream) {
+extern "C" mc_status mc_kv4_attention(const mc_kv4_attention_args* args, int32_t device, void* stream) {
+  if (!args) return set_error(MC_E_INVALID, "null pointer");
+  const void *q = args->q, *pool = args->pool;
+  const int32_t *table = args->table, *kv_len = args->kv_len, *cu_q = args->cu_q;
+  void *out = args->out, *workspace = args->workspace;
+  const int64_t q_tok = args->q_tok, q_head = args->q_head, n_pages = args->n_pages,
+                workspace_bytes = args->workspace_bytes;
+  const int32_t dtype = args->dtype, n_tokens = args->n_tokens, n_heads = args->n_heads,
+                n_kv_heads = args->n_kv_heads, head_dim = args->head_dim, table_width = args->table_width,
+                n_requests = args->n_requests;
+  const float scale = args->scale;
   if (head_dim != 64 && head_dim != 128) return set_error(MC_E_SHAPE, "head dim must be 64 or 128");
   if (n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads)
     return set_error(MC_E_SHAPE, "heads must be a multiple of the key/value heads");

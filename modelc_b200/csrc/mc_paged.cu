@@ -69,8 +69,8 @@ __global__ void __launch_bounds__(kSlotThreads) k_paged_slots(const SlotArgs a) 
       kv = max(a.kv_len[z], 0);
       q = max(a.q_len[z], 0);
     }
-    const int have = min((kv + a.page - 1) / a.page, a.width);
-    const int need = min((kv + q + a.page - 1) / a.page, a.width);
+    const int have = (int)min(((long long)kv + a.page - 1) / a.page, (long long)a.width);
+    const int need = (int)min(((long long)kv + q + a.page - 1) / a.page, (long long)a.width);
     int tok = q, pg = need - have;  // inclusive sums over the chunk
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kSlotThreads) k_paged_slots(const SlotArgs a) 
       int page = -1;
       if (j < a.width) {
         int* entry = a.table + (size_t)(z0 + l) * a.width + j;
-        if (j >= (kvl + a.page - 1) / a.page) {
+        if ((long long)j * a.page >= kvl) {
           const long long nth = (long long)n_free - 1 - (base_pg + s_start[l] + j);
           if (nth >= 0 && nth < a.n_pages_free) page = a.free_pages[nth];
           if (pos % a.page == 0) *entry = page;
@@ -393,12 +393,13 @@ struct Read {
 using namespace mc;
 
 // ------------------------------------------------------------------ C entries
-extern "C" mc_status mc_paged_slots(const int32_t* kv_len, const int32_t* q_len, int32_t n_requests,
-                                    int32_t* table, int32_t table_width, const int32_t* free_pages,
-                                    int32_t n_free_pages, const int32_t* n_free, int32_t page_size,
-                                    int32_t n_tokens, int32_t* cu_q, int32_t* positions,
-                                    int32_t* slots, int32_t* new_len, int32_t* n_free_out,
-                                    int32_t device, void* stream) {
+extern "C" mc_status mc_paged_slots(const mc_slots_args* args, int32_t device, void* stream) {
+  if (!args) return set_error(MC_E_INVALID, "null pointer");
+  const int32_t *kv_len = args->kv_len, *q_len = args->q_len, *free_pages = args->free_pages,
+                *n_free = args->n_free;
+  int32_t *table = args->table, *cu_q = args->cu_q, *positions = args->positions, *slots = args->slots, *new_len = args->new_len, *n_free_out = args->n_free_out;
+  const int32_t n_requests = args->n_requests, table_width = args->table_width,
+                n_free_pages = args->n_free_pages, page_size = args->page_size, n_tokens = args->n_tokens;
   if (n_requests < 0 || n_tokens < 0 || table_width < 0 || n_free_pages < 0)
     return set_error(MC_E_INVALID, "negative size");
   if (page_size <= 0) return set_error(MC_E_SHAPE, "page size must be positive");
@@ -409,7 +410,7 @@ extern "C" mc_status mc_paged_slots(const int32_t* kv_len, const int32_t* q_len,
   MC_PCKS(paged_device(device));
   SlotArgs a{kv_len, q_len, table, free_pages, n_free, cu_q, positions, slots, new_len, n_free_out,
              n_requests, table_width, page_size, n_tokens, n_free_pages};
-  const int grid = std::max(1, std::min(paged_sms(device), (n_tokens + kSlotThreads - 1) / kSlotThreads));
+  const int grid = std::max(1, std::min(paged_sms(device), n_tokens / kSlotThreads + 1));
   k_paged_slots<<<grid, kSlotThreads, 0, (cudaStream_t)stream>>>(a);
   MC_PCK(cudaGetLastError());
   return MC_OK;
@@ -430,12 +431,16 @@ extern "C" mc_status mc_rope_table(const double* freq, int32_t n_freq, int32_t p
 
 static size_t act_size(int t) { return t == MC_ACT_F32 ? 4 : 2; }
 
-extern "C" mc_status mc_rope(const void* q, int64_t q_tok, int64_t q_head, int32_t n_heads,
-                             const void* k, int64_t k_tok, int64_t k_head, int32_t n_kv_heads,
-                             int32_t dtype, int32_t n_tokens, int32_t head_dim, int32_t rot,
-                             int32_t interleaved, const int32_t* positions, const float* cos_table,
-                             const float* sin_table, int32_t table_rows, void* q_out, void* k_out,
-                             int32_t out_dtype, int32_t device, void* stream) {
+extern "C" mc_status mc_rope(const mc_rope_args* args, int32_t device, void* stream) {
+  if (!args) return set_error(MC_E_INVALID, "null pointer");
+  const void *q = args->q, *k = args->k;
+  const int32_t *positions = args->positions;
+  const float *cos_table = args->cos_table, *sin_table = args->sin_table;
+  void *q_out = args->q_out, *k_out = args->k_out;
+  const int64_t q_tok = args->q_tok, q_head = args->q_head, k_tok = args->k_tok, k_head = args->k_head;
+  const int32_t n_heads = args->n_heads, n_kv_heads = args->n_kv_heads, dtype = args->dtype,
+                out_dtype = args->out_dtype, n_tokens = args->n_tokens, head_dim = args->head_dim,
+                rot = args->rot, interleaved = args->interleaved, table_rows = args->table_rows;
   if (n_tokens < 0 || n_heads < 0 || n_kv_heads < 0) return set_error(MC_E_INVALID, "negative size");
   if (head_dim <= 0 || head_dim % 2 || rot <= 0 || rot % 2 || rot > head_dim)
     return set_error(MC_E_SHAPE, "rot must be even and positive, at most the (even) head dim");
@@ -491,11 +496,15 @@ extern "C" int64_t mc_kv4_page_bytes(int32_t head_dim) {
   return head_dim == 64 || head_dim == 128 ? kv4_page_bytes(head_dim) : 0;
 }
 
-extern "C" mc_status mc_kv4_append(void* pool, int64_t n_pages, int32_t n_kv_heads, int32_t head_dim,
-                                   const void* k, int64_t k_tok, int64_t k_head, const void* v,
-                                   int64_t v_tok, int64_t v_head, int32_t dtype,
-                                   const int32_t* slots, int32_t n_tokens, int32_t device,
-                                   void* stream) {
+extern "C" mc_status mc_kv4_append(const mc_kv4_append_args* args, int32_t device, void* stream) {
+  if (!args) return set_error(MC_E_INVALID, "null pointer");
+  void *pool = args->pool;
+  const void *k = args->k, *v = args->v;
+  const int32_t *slots = args->slots;
+  const int64_t n_pages = args->n_pages, k_tok = args->k_tok, k_head = args->k_head, v_tok = args->v_tok,
+                v_head = args->v_head;
+  const int32_t n_kv_heads = args->n_kv_heads, head_dim = args->head_dim, dtype = args->dtype,
+                n_tokens = args->n_tokens;
   MC_PCKS(check_pool(pool, n_pages, n_kv_heads, head_dim));
   if (dtype < 0 || dtype > 2) return set_error(MC_E_DTYPE, "unknown type");
   if (n_tokens < 0) return set_error(MC_E_INVALID, "negative size");
@@ -511,9 +520,14 @@ extern "C" mc_status mc_kv4_append(void* pool, int64_t n_pages, int32_t n_kv_hea
   return MC_OK;
 }
 
-extern "C" mc_status mc_kv4_read(const void* pool, int64_t n_pages, int32_t n_kv_heads,
-                                 int32_t head_dim, const int32_t* slots, int32_t n_tokens, void* k_out,
-                                 void* v_out, int32_t dtype, int32_t device, void* stream) {
+extern "C" mc_status mc_kv4_read(const mc_kv4_read_args* args, int32_t device, void* stream) {
+  if (!args) return set_error(MC_E_INVALID, "null pointer");
+  const void *pool = args->pool;
+  const int32_t *slots = args->slots;
+  void *k_out = args->k_out, *v_out = args->v_out;
+  const int64_t n_pages = args->n_pages;
+  const int32_t n_kv_heads = args->n_kv_heads, head_dim = args->head_dim, dtype = args->dtype,
+                n_tokens = args->n_tokens;
   MC_PCKS(check_pool(pool, n_pages, n_kv_heads, head_dim));
   if (dtype < 0 || dtype > 2) return set_error(MC_E_DTYPE, "unknown type");
   if (n_tokens < 0) return set_error(MC_E_INVALID, "negative size");

@@ -1,8 +1,12 @@
 // mc_prompt_attn.cu -- attention over whole packed prompts.
 //
 // O = softmax(scale Q K^T) V per sequence and head, one pass over the keys.
-// A block takes 256 query rows of one head as two tiles of 128 and walks the
-// keys in tiles of 128:
+// A block takes two tiles of 128 query rows and walks their keys in tiles of
+// 128.  The tiles are the same rows of two heads of one key/value head where
+// the groups have an even number of heads, so that both have the same keys,
+// and 256 rows of one head otherwise (adjacent rows for all: the second tile's
+// additional keys under a causal mask leave the first idle, and short
+// sequences the second).
 //   - one thread loads Q once and K, V tiles through a shared-memory ring
 //     (cp.async.bulk.tensor, 128-byte swizzle);
 //   - one thread issues tcgen05.mma: S = Q K^T of a tile into tensor memory,
@@ -40,6 +44,7 @@ struct PromptArgs {
   void* out;              // [Tq][H][D]
   const int *cu_q, *cu_k;
   int Tq, Tk, H, Hk, B, causal;
+  int pair, rows, units;  // tiles of two heads; rows of a block; blocks over the same rows
   float scale;
 };
 
@@ -147,9 +152,9 @@ __device__ __forceinline__ bool bar_wait_far(uint64_t* b, uint32_t parity) {
 }
 
 struct PromptWork {
-  int q0, n_q;     // first query row of the block's 256 and how many the sequence has from there
+  int q0, n_q;     // first query row of the block and how many the sequence has from there
   int k0, L;       // first key, keys
-  int shift;       // a row i of the 256 sees the keys below i + shift (causal)
+  int shift;       // row i of the block sees the keys below i + shift (causal)
   int ok;          // there is work
 };
 
@@ -165,7 +170,7 @@ __device__ __forceinline__ void prompt_work(const PromptArgs& a, int index, Prom
       const int c0 = min(max(a.cu_q[z], 0), a.Tq);
       n = max(min(a.cu_q[z + 1], a.Tq) - c0, 0);
     }
-    total += __reduce_add_sync(~0u, (n + 255) / 256);
+    total += __reduce_add_sync(~0u, (n + a.rows - 1) / a.rows);
   }
   if (lane == 0) w->ok = 0;
   __syncwarp();
@@ -179,7 +184,7 @@ __device__ __forceinline__ void prompt_work(const PromptArgs& a, int index, Prom
       c0 = min(max(a.cu_q[z], 0), a.Tq);
       n = max(min(a.cu_q[z + 1], a.Tq) - c0, 0);
     }
-    const int mine = (n + 255) / 256;
+    const int mine = (n + a.rows - 1) / a.rows;
     int inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -188,7 +193,7 @@ __device__ __forceinline__ void prompt_work(const PromptArgs& a, int index, Prom
     }
     const int first = seen + inc - mine;
     if (want >= first && want < first + mine) {
-      const int r = (want - first) * 256;
+      const int r = (want - first) * a.rows;
       const int k0 = min(max(a.cu_k[z], 0), a.Tk), k1 = max(min(a.cu_k[z + 1], a.Tk), k0);
       w->q0 = c0 + r;
       w->n_q = n - r;
@@ -258,7 +263,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   __shared__ int s_fail;
   __shared__ PromptWork s_work;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int head = blockIdx.x % a.H, index = blockIdx.x / a.H;
+  const int index = blockIdx.x / a.units, unit = blockIdx.x % a.units;
+  // tile t has the rows from t * row_1 of head + t * pair
+  const int head = a.pair ? 2 * unit : unit, row_1 = a.pair ? 0 : kPromptRows;
 
   // rows of no sequence are 0: each block clears its share
   {
@@ -297,8 +304,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   int lim[2], n_t[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const int rows = min(max(w.n_q - t * kPromptRows, 0), kPromptRows);
-    lim[t] = rows ? min(max(t * kPromptRows + rows - 1 + w.shift, 0), w.L) : 0;
+    const int rows = min(max(w.n_q - t * row_1, 0), kPromptRows);
+    lim[t] = rows ? min(max(t * row_1 + rows - 1 + w.shift, 0), w.L) : 0;
     n_t[t] = (lim[t] + kPromptRows - 1) / kPromptRows;
   }
   const int n_max = max(n_t[0], n_t[1]);
@@ -324,7 +331,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (n_t[t]) {
           bar_expect(&b_q[t], C::Tile);
           for (int h = 0; h < NH; ++h)
-            load_tile(sq + t * C::Tile + h * C::Half, &mq, h * 64, head, w.q0 + t * kPromptRows, &b_q[t]);
+            load_tile(sq + t * C::Tile + h * C::Half, &mq, h * 64, head + t * a.pair,
+                      w.q0 + t * row_1, &b_q[t]);
         }
         if (t == 0) load_k(0);
       }
@@ -425,7 +433,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // --------------------------------------------------------- softmax
-    const int t = warp >> 2, row = t * kPromptRows + (warp & 3) * 32 + lane;
+    const int t = warp >> 2, first = t * row_1 + (warp & 3) * 32, row = first + lane, head_t = head + t * a.pair;
     const uint32_t base = tmem + ((uint32_t)(warp & 3) << 21);  // the warp's 32 lanes
     const uint32_t ts = base + t * 128, to = base + C::O + t * D;
     const int n = n_t[t];
@@ -523,23 +531,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               make_uint4(y[4 * x], y[4 * x + 1], y[4 * x + 2], y[4 * x + 3]);
       }
       __syncwarp();
-      const int first = t * kPromptRows + (warp & 3) * 32;
 #pragma unroll 4
       for (int i = lane; i < 32 * (D / 8); i += 32) {
         const int r = i / (D / 8), x = i % (D / 8);
         if (first + r < w.n_q)
-          *(uint4*)((T*)a.out + ((size_t)(w.q0 + first + r) * a.H + head) * D + x * 8) =
+          *(uint4*)((T*)a.out + ((size_t)(w.q0 + first + r) * a.H + head_t) * D + x * 8) =
               *(const uint4*)(stage + r * D * 2 + ((x ^ r) % (D / 8)) * 16);
       }
     } else if (live) {  // no keys; or a wait ran out
-      T* out = (T*)a.out + ((size_t)(w.q0 + row) * a.H + head) * D;
+      T* out = (T*)a.out + ((size_t)(w.q0 + row) * a.H + head_t) * D;
       const uint32_t y = ok ? 0u : 0x7fff7fffu;
       for (int x = 0; x < D / 8; ++x) *(uint4*)(out + x * 8) = make_uint4(y, y, y, y);
     }
     __syncwarp();
     for (unsigned again = __ballot_sync(~0u, bad && live); again; again &= again - 1) {
       const int r = __ffs(again) - 1;
-      prompt_row<T, D>(a, w.q0 + t * kPromptRows + (warp & 3) * 32 + r, head, w.k0, __shfl_sync(~0u, see, r));
+      prompt_row<T, D>(a, w.q0 + first + r, head_t, w.k0, __shfl_sync(~0u, see, r));
     }
     tm_before();
   }
@@ -601,13 +608,17 @@ static cudaError_t run_prompt(const PromptArgs& a, const CUtensorMap& q, const C
 
 using namespace mc;
 
-extern "C" mc_status mc_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void* k,
-                                         int64_t k_tok, int64_t k_head, const void* v, int64_t v_tok,
-                                         int64_t v_head, int32_t dtype, int32_t n_q, int32_t n_k,
-                                         int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
-                                         const int32_t* cu_q, const int32_t* cu_k,
-                                         int32_t n_sequences, float scale, int32_t causal, void* out,
-                                         int32_t device, void* stream) {
+extern "C" mc_status mc_prompt_attention(const mc_prompt_args* args, int32_t device, void* stream) {
+  if (!args) return set_error(MC_E_INVALID, "null pointer");
+  const void *q = args->q, *k = args->k, *v = args->v;
+  const int32_t *cu_q = args->cu_q, *cu_k = args->cu_k;
+  void *out = args->out;
+  const int64_t q_tok = args->q_tok, q_head = args->q_head, k_tok = args->k_tok, k_head = args->k_head,
+                v_tok = args->v_tok, v_head = args->v_head;
+  const int32_t dtype = args->dtype, n_q = args->n_q, n_k = args->n_k, n_heads = args->n_heads,
+                n_kv_heads = args->n_kv_heads, head_dim = args->head_dim, n_sequences = args->n_sequences,
+                causal = args->causal;
+  const float scale = args->scale;
   if (head_dim != 64 && head_dim != 128) return set_error(MC_E_SHAPE, "head dim must be 64 or 128");
   if (n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads)
     return set_error(MC_E_SHAPE, "heads must be a multiple of the key/value heads");
@@ -622,8 +633,11 @@ extern "C" mc_status mc_prompt_attention(const void* q, int64_t q_tok, int64_t q
     return set_error(MC_E_INVALID, "rows must be 16-byte aligned");
   if (q_tok < 0 || q_head < 0 || k_tok < 0 || k_head < 0 || v_tok < 0 || v_head < 0)
     return set_error(MC_E_INVALID, "negative stride");
-  const long long blocks = ((long long)(n_q + 255) / 256 + n_sequences) * n_heads;
-  if (blocks > 0x7fffffffll) return set_error(MC_E_CAPACITY, "too many rows for one call");
+  const int pair = n_heads / n_kv_heads % 2 == 0, rows = pair ? kPromptRows : 2 * kPromptRows;
+  const int units = pair ? n_heads / 2 : n_heads;
+  const long long blocks = (((long long)n_q + rows - 1) / rows + n_sequences) * units;
+  if (blocks > 0x7fffffffll || n_q > 0x7fffff00 || n_k > 0x7fffff00)
+    return set_error(MC_E_CAPACITY, "too many rows for one call");
   MC_PCKS(paged_device(device));
   cudaStream_t s = (cudaStream_t)stream;
   if (n_k == 0 || n_sequences == 0) {  // no row sees a key
@@ -631,7 +645,7 @@ extern "C" mc_status mc_prompt_attention(const void* q, int64_t q_tok, int64_t q
     return MC_OK;
   }
   PromptArgs a{q, k, v, q_tok, q_head, k_tok, k_head, v_tok, v_head, out, cu_q, cu_k, n_q, n_k,
-               n_heads, n_kv_heads, n_sequences, causal, scale};
+               n_heads, n_kv_heads, n_sequences, causal, pair, rows, units, scale};
   CUtensorMap mq, mk, mv;
   const bool bf = dtype == MC_ACT_BF16;
   if (!head_map(&mq, bf, q, head_dim, n_heads, n_q, q_tok, q_head) ||

@@ -6,11 +6,18 @@ one asynchronous call of the C ABI (include/modelc_cuda.h) on the current
 stream of the tensors' device; the arithmetic is described there.  Tensors
 used on another stream than the one they were allocated on need torch's usual
 care (record_stream or events).
+
+Decode steps make these calls with a few tokens each, where the host's time is
+the whole cost: the argument structs are packed with ``struct`` and passed as
+one pointer (0.8 us where ctypes took 2.2 us for 22 arguments), and the stream
+is asked for as a number (0.1 us where the Stream object took 2.2 us).
 """
 from __future__ import annotations
 
 import math
+import threading
 from dataclasses import dataclass
+from struct import Struct
 from typing import NamedTuple
 
 import torch
@@ -21,43 +28,60 @@ from ._lib import check, lib
 PAGE = 64  # tokens of a page of the 4-bit cache
 
 _ACT = {torch.float32: _lib.ACT_F32, torch.float16: _lib.ACT_F16, torch.bfloat16: _lib.ACT_BF16}
-_HALF = (torch.float16, torch.bfloat16)
+_INT, _F32, _F16, _BF16 = torch.int32, torch.float32, torch.float16, torch.bfloat16
+
+# mc_slots_args, mc_rope_args, ... in the C compiler's layout
+_SLOTS = Struct("@10P5i").pack
+_ROPE = Struct("@7P4q9i").pack
+_APPEND = Struct("@4P5q4i").pack
+_READ = Struct("@4Pq4i").pack
+_ATTENTION = Struct("@7P4q7if").pack
+_PROMPT = Struct("@6P6q8if").pack
 
 
-def _index(t: torch.Tensor, name: str, device, shape=None) -> int:
-    """Pointer of a contiguous int32 tensor on `device`."""
-    if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name}: a contiguous int32 tensor on {device} is wanted")
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the same number without the Stream object around it
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+
+def _index(t: torch.Tensor, name: str, dev: int, shape=None) -> int:
+    """Pointer of a contiguous int32 tensor on CUDA device `dev`."""
+    if t.dtype is not _INT or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous int32 tensor on cuda:{dev} is wanted")
     if shape is not None and t.shape != shape:
         raise ValueError(f"{name}: shape {tuple(t.shape)}, {tuple(shape)} is wanted")
     return t.data_ptr()
 
 
-def _heads(t: torch.Tensor, name: str, device) -> torch.Tensor:
-    """[tokens, heads, head_dim] on `device` with a contiguous last axis."""
-    if t.dim() != 3 or t.device != device or t.dtype not in _ACT:
-        raise ValueError(f"{name}: [tokens, heads, head_dim] of f32, f16 or bf16 on {device} is wanted")
+def _heads(t: torch.Tensor, name: str, dev: int) -> torch.Tensor:
+    """[tokens, heads, head_dim] on device `dev` with a contiguous last axis."""
+    if t.dim() != 3 or t.get_device() != dev or t.dtype not in _ACT:
+        raise ValueError(f"{name}: [tokens, heads, head_dim] of f32, f16 or bf16 on cuda:{dev} is wanted")
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
 def _rows16(t: torch.Tensor):
     """f16 or bf16 rows whose every head starts at a multiple of 16 bytes (a
     copy where they do not), with their token and head strides."""
-    s = t.stride()
-    if s[0] <= 0 or s[1] <= 0 or (s[0] | s[1]) % 8 or t.data_ptr() % 16:
+    s0, s1, _ = t.stride()
+    if s0 <= 0 or s1 <= 0 or (s0 | s1) % 8 or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
         return t, t.shape[1] * t.shape[2], t.shape[2]
-    return t, s[0], s[1]
+    return t, s0, s1
 
 
-def _gpu(t: torch.Tensor, name: str):
-    if not t.is_cuda:
+def _gpu(t: torch.Tensor, name: str) -> int:
+    dev = t.get_device()
+    if dev < 0:
         raise ValueError(f"{name}: a CUDA tensor is wanted")
-    return t.device
+    return dev
 
 
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def _like(t: torch.Tensor, dtype=None) -> torch.Tensor:
+    return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
 
 
 class PagedStep(NamedTuple):
@@ -80,13 +104,18 @@ def paged_slots(kv_len, q_len, table, free_pages, n_free, tokens: int, page_size
         raise ValueError(f"table: [{n}, width] is wanted")
     if tokens < 0:
         raise ValueError("tokens: negative")
-    args = (_index(kv_len, "kv_len", dev), _index(q_len, "q_len", dev, kv_len.shape), n,
-            _index(table, "table", dev), table.shape[1], _index(free_pages, "free_pages", dev),
-            free_pages.numel(), _index(n_free, "n_free", dev, (1,)), page_size, tokens)
-    out = torch.empty(2 * (tokens + n + 1), dtype=torch.int32, device=dev)
-    step = PagedStep(*out.split_with_sizes((n + 1, tokens, tokens, n, 1)))
-    check(lib().mc_paged_slots(*args, *(t.data_ptr() for t in step), dev.index, _stream(dev)))
-    return step
+    kv = _index(kv_len, "kv_len", dev)
+    q = _index(q_len, "q_len", dev, kv_len.shape)
+    tab = _index(table, "table", dev)
+    free = _index(free_pages, "free_pages", dev)
+    left = _index(n_free, "n_free", dev, (1,))
+    out = torch.empty(2 * (tokens + n + 1), dtype=_INT, device=kv_len.device)
+    p = out.data_ptr()  # cu_q, positions, slots, new_len, n_free one behind the other
+    pos = p + 4 * (n + 1)
+    new = pos + 8 * tokens
+    check(lib().mc_paged_slots(_SLOTS(kv, q, tab, free, left, p, pos, pos + 4 * tokens, new, new + 4 * n, n,
+                                      table.shape[1], free_pages.shape[0], page_size, tokens), dev, _stream(dev)))
+    return PagedStep(*out.unsafe_split_with_sizes((n + 1, tokens, tokens, n, 1)))
 
 
 # --------------------------------------------------------- rotary positions
@@ -143,10 +172,11 @@ def rope_table(positions: int, rot: int, theta: float = 10000.0,
     dev = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
     f, factor = rope_frequencies(rot, theta, scaling)
     freq = torch.tensor(f, dtype=torch.float64, device=dev)
-    cos = torch.empty((positions, rot // 2), dtype=torch.float32, device=dev)
+    cos = torch.empty((positions, rot // 2), dtype=_F32, device=dev)
     sin = torch.empty_like(cos)
+    dev = cos.get_device()
     check(lib().mc_rope_table(freq.data_ptr(), len(f), positions, factor, cos.data_ptr(),
-                              sin.data_ptr(), cos.device.index, _stream(cos.device)))
+                              sin.data_ptr(), dev, _stream(dev)))
     return cos, sin
 
 
@@ -158,29 +188,31 @@ def rope(q, k, positions, cos, sin, layout: str = "half", dtype=None):
     dev = _gpu(q, "q")
     q = _heads(q, "q", dev)
     T, H, D = q.shape
-    if layout not in ("half", "interleaved"):
+    if layout != "half" and layout != "interleaved":
         raise ValueError(f"unknown layout {layout!r}")
-    if cos.shape != sin.shape or cos.dim() != 2 or cos.dtype != torch.float32 or sin.dtype != torch.float32 \
-            or not (cos.is_contiguous() and sin.is_contiguous()) or cos.device != dev or sin.device != dev:
-        raise ValueError(f"cos, sin: contiguous f32 [positions, rot/2] on {dev} are wanted")
-    dtype = dtype or q.dtype
+    if cos.shape != sin.shape or cos.dim() != 2 or cos.dtype is not _F32 or sin.dtype is not _F32 \
+            or not (cos.is_contiguous() and sin.is_contiguous()) or cos.get_device() != dev \
+            or sin.get_device() != dev:
+        raise ValueError(f"cos, sin: contiguous f32 [positions, rot/2] on cuda:{dev} are wanted")
+    own = q.dtype
+    dtype = dtype or own
     if dtype not in _ACT:
         raise ValueError("dtype: f32, f16 or bf16 is wanted")
     pos = _index(positions, "positions", dev, (T,))
-    qo = torch.empty((T, H, D), dtype=dtype, device=dev)
-    ko, Hk, kp, ks = None, 0, None, (0, 0, 0)
+    qo = _like(q, dtype)
+    ko, Hk, kp, kop, k0, k1 = None, 0, 0, 0, 0, 0
     if k is not None:
         k = _heads(k, "k", dev)
-        if k.shape[0] != T or k.shape[2] != D or k.dtype != q.dtype:
+        if k.shape[0] != T or k.shape[2] != D or k.dtype is not own:
             raise ValueError("k: q's tokens, head dim and type are wanted")
-        Hk, ks, kp = k.shape[1], k.stride(), k.data_ptr()
-        ko = torch.empty((T, Hk, D), dtype=dtype, device=dev)
-    qs = q.stride()
-    check(lib().mc_rope(q.data_ptr(), qs[0], qs[1], H, kp, ks[0], ks[1], Hk, _ACT[q.dtype], T, D,
-                        2 * cos.shape[1], layout == "interleaved", pos, cos.data_ptr(),
-                        sin.data_ptr(), cos.shape[0], qo.data_ptr(),
-                        ko.data_ptr() if ko is not None else None, _ACT[dtype], dev.index,
-                        _stream(dev)))
+        ko = _like(k, dtype)
+        Hk, kp, kop = k.shape[1], k.data_ptr(), ko.data_ptr()
+        k0, k1, _ = k.stride()
+    q0, q1, _ = q.stride()
+    rows, half = cos.shape
+    check(lib().mc_rope(_ROPE(q.data_ptr(), kp, pos, cos.data_ptr(), sin.data_ptr(), qo.data_ptr(), kop, q0, q1,
+                              k0, k1, H, Hk, _ACT[own], _ACT[dtype], T, D, 2 * half, layout == "interleaved",
+                              rows), dev, _stream(dev)))
     return qo, ko
 
 
@@ -195,11 +227,12 @@ def kv4_pool(n_pages: int, n_kv_heads: int, head_dim: int, device=0) -> torch.Te
     return torch.zeros((n_pages, n_kv_heads, n), dtype=torch.uint8, device=dev)
 
 
-def _pool(pool: torch.Tensor, head_dim: int):
-    if pool.dim() != 3 or pool.dtype != torch.uint8 or not pool.is_contiguous() or not pool.is_cuda \
+def _pool(pool: torch.Tensor, head_dim: int) -> int:
+    dev = pool.get_device()
+    if pool.dim() != 3 or pool.dtype is not torch.uint8 or dev < 0 or not pool.is_contiguous() \
             or pool.shape[2] != 72 * head_dim:
         raise ValueError("pool: a contiguous uint8 [pages, kv heads, 72 * head_dim] CUDA tensor is wanted")
-    return pool.device
+    return dev
 
 
 def kv4_append(pool, k, v, slots) -> None:
@@ -208,12 +241,13 @@ def kv4_append(pool, k, v, slots) -> None:
     dev = _pool(pool, k.shape[-1])
     k, v = _heads(k, "k", dev), _heads(v, "v", dev)
     T, Hk, D = k.shape
-    if v.shape != k.shape or v.dtype != k.dtype or Hk != pool.shape[1]:
+    if v.shape != k.shape or v.dtype is not k.dtype or Hk != pool.shape[1]:
         raise ValueError("k, v: one shape and type, and the pool's heads, are wanted")
-    ks, vs = k.stride(), v.stride()
-    check(lib().mc_kv4_append(pool.data_ptr(), pool.shape[0], Hk, D, k.data_ptr(), ks[0], ks[1],
-                              v.data_ptr(), vs[0], vs[1], _ACT[k.dtype],
-                              _index(slots, "slots", dev, (T,)), T, dev.index, _stream(dev)))
+    k0, k1, _ = k.stride()
+    v0, v1, _ = v.stride()
+    check(lib().mc_kv4_append(_APPEND(pool.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                      _index(slots, "slots", dev, (T,)), pool.shape[0], k0, k1, v0, v1, Hk, D,
+                                      _ACT[k.dtype], T), dev, _stream(dev)))
 
 
 def kv4_read(pool, slots, head_dim: int, dtype=torch.bfloat16):
@@ -222,12 +256,36 @@ def kv4_read(pool, slots, head_dim: int, dtype=torch.bfloat16):
     if dtype not in _ACT:
         raise ValueError("dtype: f32, f16 or bf16 is wanted")
     T, Hk = slots.numel(), pool.shape[1]
-    out = torch.empty((2, T, Hk, head_dim), dtype=dtype, device=dev)
-    k, v = out.unbind(0)
-    check(lib().mc_kv4_read(pool.data_ptr(), pool.shape[0], Hk, head_dim,
-                            _index(slots, "slots", dev), T, k.data_ptr(), v.data_ptr(),
-                            _ACT[dtype], dev.index, _stream(dev)))
+    k = torch.empty((T, Hk, head_dim), dtype=dtype, device=pool.device)
+    v = torch.empty_like(k)
+    check(lib().mc_kv4_read(_READ(pool.data_ptr(), _index(slots, "slots", dev), k.data_ptr(), v.data_ptr(),
+                                  pool.shape[0], Hk, head_dim, _ACT[dtype], T), dev, _stream(dev)))
     return k, v
+
+
+# Workspaces of kv4_attention, one per device, stream and host thread: calls
+# of one thread on one stream run one after the other, so they can share it.
+# A call that is captured into a graph gets one of its own, from the graph's
+# memory: the graph may run on any stream.
+_workspaces: dict = {}
+
+
+def _workspace(dev: int, stream: int, requests: int, head_dim: int):
+    if torch.cuda.is_current_stream_capturing():
+        n = lib().mc_kv4_attention_workspace(requests, head_dim, dev)
+        return torch.empty(max(n, 0), dtype=torch.uint8, device=torch.device("cuda", dev)), n
+    key = (dev, stream, threading.get_ident())
+    kept = _workspaces.get(key)
+    if kept is not None and requests <= kept[1] and head_dim <= kept[2]:
+        return kept[0], kept[3]
+    if kept is not None:
+        requests, head_dim = max(requests, kept[1]), max(head_dim, kept[2])
+    n = lib().mc_kv4_attention_workspace(requests, head_dim, dev)
+    if n <= 0:
+        raise ValueError(f"head dim {head_dim}: 64 or 128 is wanted")
+    ws = torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", dev))
+    _workspaces[key] = (ws, requests, head_dim, n)
+    return ws, n
 
 
 def kv4_attention(q, pool, table, kv_len, cu_q, scale: float | None = None):
@@ -241,20 +299,21 @@ def kv4_attention(q, pool, table, kv_len, cu_q, scale: float | None = None):
     T, H, D = q.shape
     if _pool(pool, D) != dev:
         raise ValueError("q, pool: on different devices")
-    if q.dtype not in _HALF:
+    dt = q.dtype
+    if dt is not _BF16 and dt is not _F16:
         raise ValueError("q: f16 or bf16 is wanted")
     B = kv_len.shape[0]
     if table.dim() != 2 or table.shape[0] != B:
         raise ValueError(f"table: [{B}, width] is wanted")
-    Hk = pool.shape[1]
-    out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
-    ws = torch.empty(lib().mc_kv4_attention_workspace(B, D, dev.index), dtype=torch.uint8, device=dev)
-    qs = q.stride()
-    check(lib().mc_kv4_attention(q.data_ptr(), qs[0], qs[1], _ACT[q.dtype], T, H, pool.data_ptr(),
-                                 pool.shape[0], Hk, D, _index(table, "table", dev), table.shape[1],
-                                 _index(kv_len, "kv_len", dev), _index(cu_q, "cu_q", dev, (B + 1,)),
-                                 B, D ** -0.5 if scale is None else scale, out.data_ptr(),
-                                 ws.data_ptr(), ws.numel(), dev.index, _stream(dev)))
+    pages, Hk, _ = pool.shape
+    out = _like(q)
+    stream = _stream(dev)
+    ws, n = _workspace(dev, stream, B, D)
+    q0, q1, _ = q.stride()
+    check(lib().mc_kv4_attention(_ATTENTION(
+        q.data_ptr(), pool.data_ptr(), _index(table, "table", dev), _index(kv_len, "kv_len", dev),
+        _index(cu_q, "cu_q", dev, (B + 1,)), out.data_ptr(), ws.data_ptr(), q0, q1, pages, n, _ACT[dt], T, H, Hk,
+        D, table.shape[1], B, D ** -0.5 if scale is None else scale), dev, stream))
     return out
 
 
@@ -267,20 +326,20 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, scale: float | None = None, causa
     dev = _gpu(q, "q")
     q, k, v = _heads(q, "q", dev), _heads(k, "k", dev), _heads(v, "v", dev)
     T, H, D = q.shape
-    if q.dtype not in _HALF or k.dtype != q.dtype or v.dtype != q.dtype:
+    dt = q.dtype
+    if (dt is not _BF16 and dt is not _F16) or k.dtype is not dt or v.dtype is not dt:
         raise ValueError("q, k, v: one type, f16 or bf16, is wanted")
+    Tk, Hk, _ = k.shape
     if k.shape != v.shape or k.shape[2] != D:
         raise ValueError("k, v: one shape, with q's head dim, is wanted")
-    (q, qt, qh), (k, kt, kh), (v, vt, vh) = _rows16(q), _rows16(k), _rows16(v)
+    (q, q0, q1), (k, k0, k1), (v, v0, v1) = _rows16(q), _rows16(k), _rows16(v)
     cu_k = cu_q if cu_k is None else cu_k
     B = cu_q.shape[0] - 1
     if B < 0:
         raise ValueError("cu_q: [sequences + 1] is wanted")
-    out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
-    check(lib().mc_prompt_attention(q.data_ptr(), qt, qh, k.data_ptr(), kt, kh,
-                                    v.data_ptr(), vt, vh, _ACT[q.dtype], T, k.shape[0], H,
-                                    k.shape[1], D, _index(cu_q, "cu_q", dev),
-                                    _index(cu_k, "cu_k", dev, (B + 1,)), B,
-                                    D ** -0.5 if scale is None else scale, causal, out.data_ptr(),
-                                    dev.index, _stream(dev)))
+    out = _like(q)
+    check(lib().mc_prompt_attention(_PROMPT(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _index(cu_q, "cu_q", dev), _index(cu_k, "cu_k", dev, (B + 1,)),
+        out.data_ptr(), q0, q1, k0, k1, v0, v1, _ACT[dt], T, Tk, H, Hk, D, B, causal,
+        D ** -0.5 if scale is None else scale), dev, _stream(dev)))
     return out

@@ -502,56 +502,115 @@ def test_prompt_attention_nonfinite_tokens(D, what):
 
 
 # ------------------------------------------------------------------ refusals
-P = C.c_void_p(4096)  # an address that no refused call reads
+P = 4096  # an address that no refused call reads
+
+
+def _call(name, struct, device=0, **d):
+    """The C entry with a struct of these fields (pointers default to P, numbers to 0)."""
+    s = struct()
+    for field, kind in struct._fields_:
+        setattr(s, field, d.pop(field, P if kind is C.c_void_p else 0))
+    assert not d, d
+    return getattr(mb.lib(), name)(bytes(s), device, None)
+
+
+def _struct(pointers, longs, ints, floats=""):
+    class S(C.Structure):
+        _fields_ = ([(n, C.c_void_p) for n in pointers.split()] + [(n, C.c_int64) for n in longs.split()] +
+                    [(n, C.c_int32) for n in ints.split()] + [(n, C.c_float) for n in floats.split()])
+    return S
+
+
+SLOTS = _struct("kv_len q_len table free_pages n_free cu_q positions slots new_len n_free_out", "",
+                "n_requests table_width n_free_pages page_size n_tokens")
+ROPE = _struct("q k positions cos_table sin_table q_out k_out", "q_tok q_head k_tok k_head",
+               "n_heads n_kv_heads dtype out_dtype n_tokens head_dim rot interleaved table_rows")
+APPEND = _struct("pool k v slots", "n_pages k_tok k_head v_tok v_head", "n_kv_heads head_dim dtype n_tokens")
+READ = _struct("pool slots k_out v_out", "n_pages", "n_kv_heads head_dim dtype n_tokens")
+ATTENTION = _struct("q pool table kv_len cu_q out workspace", "q_tok q_head n_pages workspace_bytes",
+                    "dtype n_tokens n_heads n_kv_heads head_dim table_width n_requests", "scale")
+PROMPT = _struct("q k v cu_q cu_k out", "q_tok q_head k_tok k_head v_tok v_head",
+                 "dtype n_q n_k n_heads n_kv_heads head_dim n_sequences causal", "scale")
+
+
+def test_structs_match_the_header():
+    """Field names and order of the packed structs are the header's."""
+    import os
+    import re
+    from modelc_b200 import paged
+    txt = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include",
+                            "modelc_cuda.h")).read()
+    for name, struct, pack in (("mc_slots_args", SLOTS, paged._SLOTS), ("mc_rope_args", ROPE, paged._ROPE),
+                               ("mc_kv4_append_args", APPEND, paged._APPEND), ("mc_kv4_read_args", READ, paged._READ),
+                               ("mc_kv4_attention_args", ATTENTION, paged._ATTENTION),
+                               ("mc_prompt_args", PROMPT, paged._PROMPT)):
+        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), txt, re.S).group(1)
+        body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+        kinds = {"int64_t": C.c_int64, "int32_t": C.c_int32, "float": C.c_float}
+        fields = []
+        for line in body.split(";")[:-1]:
+            base, names = re.match(r"\s*(?:const )?(\w+)\s*(.*)", line, re.S).groups()
+            for v in names.split(","):
+                fields.append((v.strip().lstrip("*").strip(), C.c_void_p if "*" in v else kinds[base]))
+        assert [f[0] for f in fields] == [f[0] for f in struct._fields_], name
+        assert [f[1] for f in fields] == [f[1] for f in struct._fields_], name
+        values = [i if k is not C.c_float else float(i) for i, (_, k) in enumerate(struct._fields_)]
+        s = struct.from_buffer_copy(pack(*values) + bytes(8))
+        assert [getattr(s, n) or 0 for n, _ in struct._fields_] == values, name
 
 
 @pytest.mark.parametrize("status,args", [
-    (-1, dict(n=-1)), (-1, dict(tokens=-1)), (-2, dict(page=0)), (-1, dict(n_free=None)), (-1, dict(cu=None)),
-    (-1, dict(kv=None))])
+    (-1, dict(n_requests=-1)), (-1, dict(n_tokens=-1)), (-2, dict(page_size=0)), (-1, dict(n_free=None)),
+    (-1, dict(cu_q=None)), (-1, dict(kv_len=None)), (-1, dict(table=None)), (-1, dict(slots=None))])
 def test_paged_slots_refuses(status, args):
-    d = dict(n=2, tokens=4, page=64, n_free=P, cu=P, kv=P) | args
-    assert mb.lib().mc_paged_slots(d["kv"], P, d["n"], P, 4, P, 4, d["n_free"], d["page"], d["tokens"], d["cu"],
-                                   P, P, P, P, 0, None) == status
+    d = dict(n_requests=2, n_tokens=4, page_size=64, table_width=4, n_free_pages=4) | args
+    assert _call("mc_paged_slots", SLOTS, **d) == status
 
 
 @pytest.mark.parametrize("status,args", [
-    (-2, dict(rot=7)), (-2, dict(rot=130)), (-2, dict(rot=0)), (-3, dict(dt=5)), (-3, dict(dt=1, out=2)),
-    (-1, dict(T=-1)), (-1, dict(q=None)), (-2, dict(rows=0)), (-10, dict(T=1 << 30))])
+    (-2, dict(rot=7)), (-2, dict(rot=130)), (-2, dict(rot=0)), (-2, dict(head_dim=127)), (-3, dict(dtype=5)),
+    (-3, dict(dtype=1, out_dtype=2)), (-1, dict(n_tokens=-1)), (-1, dict(q=None)), (-1, dict(k_out=None)),
+    (-2, dict(table_rows=0)), (-10, dict(n_tokens=1 << 30))])
 def test_rope_refuses(status, args):
-    d = dict(rot=128, dt=0, out=0, T=4, q=P, rows=10) | args
-    assert mb.lib().mc_rope(d["q"], 1024, 128, 8, P, 1024, 128, 8, d["dt"], d["T"], 128, d["rot"], 0, P, P, P,
-                            d["rows"], P, P, d["out"], 0, None) == status
+    d = dict(rot=128, n_tokens=4, n_heads=8, n_kv_heads=8, head_dim=128, table_rows=10, q_tok=1024, q_head=128,
+             k_tok=1024, k_head=128) | args
+    assert _call("mc_rope", ROPE, **d) == status
 
 
 @pytest.mark.parametrize("status,args", [
-    (-2, dict(D=96)), (-2, dict(Hk=0)), (-10, dict(pages=1 << 26)), (-1, dict(pool=C.c_void_p(4104))),
-    (-3, dict(dt=9)), (-1, dict(T=-2)), (-1, dict(slots=None))])
+    (-2, dict(head_dim=96)), (-2, dict(n_kv_heads=0)), (-10, dict(n_pages=1 << 26)), (-1, dict(pool=4104)),
+    (-3, dict(dtype=9)), (-1, dict(n_tokens=-2)), (-1, dict(slots=None))])
 def test_kv4_append_and_read_refuse(status, args):
-    d = dict(D=128, Hk=2, pages=9, pool=P, dt=2, T=3, slots=P) | args
-    L = mb.lib()
-    assert L.mc_kv4_append(d["pool"], d["pages"], d["Hk"], d["D"], P, 1, 1, P, 1, 1, d["dt"], d["slots"], d["T"],
-                           0, None) == status
-    assert L.mc_kv4_read(d["pool"], d["pages"], d["Hk"], d["D"], d["slots"], d["T"], P, P, d["dt"], 0, None) == status
+    d = dict(head_dim=128, n_kv_heads=2, n_pages=9, dtype=2, n_tokens=3) | args
+    assert _call("mc_kv4_append", APPEND, **d) == status
+    assert _call("mc_kv4_read", READ, **d) == status
     assert _lib.last_error()
 
 
 @pytest.mark.parametrize("status,args", [
-    (-2, dict(D=80)), (-2, dict(H=5)), (-3, dict(dt=0)), (-1, dict(T=-1)), (-1, dict(q=None)),
-    (-1, dict(scale=math.inf)), (-10, dict(pages=1 << 26)), (-1, dict(pool=C.c_void_p(4104))),
-    (-1, dict(ws=None))])
+    (-2, dict(head_dim=80)), (-2, dict(n_heads=5)), (-3, dict(dtype=0)), (-1, dict(n_tokens=-1)), (-1, dict(q=None)),
+    (-1, dict(scale=math.inf)), (-10, dict(n_pages=1 << 26)), (-1, dict(pool=4104)), (-1, dict(workspace=None)),
+    (-1, dict(workspace=4100)), (-10, dict(n_tokens=1 << 30, n_heads=4))])
 def test_kv4_attention_refuses(status, args):
-    d = dict(D=128, H=4, dt=2, T=3, q=P, scale=0.1, pages=9, pool=P, ws=P) | args
-    assert mb.lib().mc_kv4_attention(d["q"], 512, 128, d["dt"], d["T"], d["H"], d["pool"], d["pages"], 2, d["D"], P,
-                                     4, P, P, 1, d["scale"], P, d["ws"], 0, 0, None) == status
+    d = dict(head_dim=128, n_heads=4, n_kv_heads=2, dtype=2, n_tokens=3, scale=0.1, n_pages=9, n_requests=1,
+             table_width=4, q_tok=512, q_head=128) | args
+    assert _call("mc_kv4_attention", ATTENTION, **d) == status
 
 
 @pytest.mark.parametrize("status,args", [
-    (-2, dict(D=96)), (-2, dict(H=3)), (-3, dict(dt=0)), (-1, dict(n=-1)), (-1, dict(v=None)),
-    (-1, dict(scale=math.nan))])
+    (-2, dict(head_dim=96)), (-2, dict(n_heads=3)), (-3, dict(dtype=0)), (-1, dict(n_q=-1)), (-1, dict(v=None)),
+    (-1, dict(scale=math.nan)), (-1, dict(k=4104)), (-1, dict(q_tok=260)), (-1, dict(v_head=-64)),
+    (-10, dict(n_q=2 ** 31 - 1, n_heads=1024))])
 def test_prompt_attention_refuses(status, args):
-    d = dict(D=64, H=4, dt=1, n=3, v=P, scale=0.1) | args
-    assert mb.lib().mc_prompt_attention(P, 256, 64, P, 128, 64, d["v"], 128, 64, d["dt"], d["n"], 3, d["H"], 2,
-                                        d["D"], P, P, 1, d["scale"], 1, P, 0, None) == status
+    d = dict(head_dim=64, n_heads=4, n_kv_heads=2, dtype=1, n_q=3, n_k=3, scale=0.1, causal=1, n_sequences=1,
+             q_tok=256, q_head=64, k_tok=128, k_head=64, v_tok=128, v_head=64) | args
+    assert _call("mc_prompt_attention", PROMPT, **d) == status
+
+
+def test_null_struct_is_refused():
+    for name in ("mc_paged_slots", "mc_rope", "mc_kv4_append", "mc_kv4_read", "mc_kv4_attention",
+                 "mc_prompt_attention"):
+        assert getattr(mb.lib(), name)(None, 0, None) == -1
 
 
 def test_page_bytes():
