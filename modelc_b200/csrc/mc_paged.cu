@@ -271,64 +271,105 @@ struct AppendArgs {
   int T, Hk, n_slots;
 };
 
-// W = D/8 lanes take one row (a token's K or V of one head); lane w holds the
-// values w, w + W, ... of its word.  A block's first value of largest size is
-// the maximum of (size, 31 - place, sign) over the W lanes.
-template <typename T, int D>
+// A row (a token's K or V of one head) is taken by D/8 lanes with 8
+// consecutive values each, so loads are 16 or 32 bytes a lane.  Word w of a
+// row holds the values w, w + W, ...: for each of the D/64 sets of 8 lanes
+// (every lane of D = 64, lanes of one parity of D = 128) lane n's code j goes
+// to word j of the set, nibble n.  That is a transposition of an 8 x 8 matrix
+// of nibbles, three exchanges with the lane 4, 2 and 1 sets away.
+template <int D>
+__device__ __forceinline__ uint32_t nibble_transpose(uint32_t x) {
+  constexpr int S = D / 64;  // lanes between neighbours of a set
+  const int n = (threadIdx.x / S) % 8;
+#pragma unroll
+  for (int k = 4; k; k >>= 1) {
+    const int sh = 4 * k;
+    const uint32_t low = k == 4 ? 0x0000ffffu : k == 2 ? 0x00ff00ffu : 0x0f0f0f0fu;
+    // lanes with bit k clear give their upper and get the other's lower parts
+    const uint32_t got = __shfl_xor_sync(~0u, n & k ? x & low : (x >> sh) & low, k * S);
+    x = n & k ? (x & low << sh) | got : (x & low) | got << sh;
+  }
+  return x;
+}
+// Even logical nibbles into the low, odd ones into the high half, and back.
+__device__ __forceinline__ uint32_t nibbles_out(uint32_t x) {
+  uint32_t e = x & 0x0f0f0f0fu, o = (x >> 4) & 0x0f0f0f0fu;
+  e = (e | e >> 4) & 0x00ff00ffu, o = (o | o >> 4) & 0x00ff00ffu;
+  e = (e | e >> 8) & 0xffffu, o = (o | o >> 8) & 0xffffu;
+  return e | o << 16;
+}
+__device__ __forceinline__ uint32_t nibbles_in(uint32_t x) {
+  uint32_t e = x & 0xffffu, o = x >> 16;
+  e = (e | e << 8) & 0x00ff00ffu, o = (o | o << 8) & 0x00ff00ffu;
+  e = (e | e << 4) & 0x0f0f0f0fu, o = (o | o << 4) & 0x0f0f0f0fu;
+  return e | o << 4;
+}
+// Word that lane n of a set holds after the transposition.
+template <int D>
+__device__ __forceinline__ int lane_word(int c) {
+  return D == 128 ? 8 * (c & 1) + (c >> 1) : c;
+}
+
+template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(256) k_kv4_append(const AppendArgs a) {
-  constexpr int W = D / 8, NB = D / 32, PB = 32 / W;  // PB: values of a block in one lane
+  constexpr int W = D / 8, NB = D / 32;
   const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / W;
-  const int w = threadIdx.x % W;
-  const long long n_rows = 2ll * a.T * a.Hk;
-  const bool live = row < n_rows;
-  const int kv = live ? (int)(row % 2) : 0;
-  const int h = live ? (int)((row / 2) % a.Hk) : 0;
-  const long long t = live ? row / 2 / a.Hk : 0;
+  const int c = threadIdx.x % W, lane = threadIdx.x & 31;
+  const bool live = row < 2ll * a.T * a.Hk;
+  const uint32_t th = live ? (uint32_t)(row / 2) : 0u;  // T Hk < 2^31
+  const int kv = (int)(row & 1), h = (int)(th % (uint32_t)a.Hk);
+  const long long t = th / (uint32_t)a.Hk;
   const int slot = live ? a.slots[t] : -1;
+  const bool on = slot >= 0 && slot < a.n_slots;
   float x[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = 0.f;
-  if (slot >= 0 && slot < a.n_slots) {
-    const T* p = kv ? (const T*)a.v + t * a.v_tok + h * a.v_head
-                    : (const T*)a.k + t * a.k_tok + h * a.k_head;
+  if (on) {
+    const T* p = (kv ? (const T*)a.v + t * a.v_tok + h * a.v_head : (const T*)a.k + t * a.k_tok + h * a.k_head) + 8 * c;
+    if (VEC) {
+      const Pack<T, 16 / sizeof(T)>* v = (const Pack<T, 16 / sizeof(T)>*)p;
+      Pack<T, 16 / sizeof(T)> y[sizeof(T) / 2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f(p[i * W + w]);
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) y[i] = v[i];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = to_f(y[i / (16 / sizeof(T))].x[i % (16 / sizeof(T))]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = to_f(p[i]);
+    }
   }
+  // the block's largest size over its 4 lanes (a NaN stays one), then the
+  // first value that has it
+  float top = fabsf(x[0]);
+#pragma unroll
+  for (int i = 1; i < 8; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(x[i])));
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    const float y = __shfl_xor_sync(~0u, top, o);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(y));
+  }
+  float mine = top;
+  bool has = false;
+#pragma unroll
+  for (int i = 7; i >= 0; --i)
+    if (fabsf(x[i]) == top) mine = x[i], has = true;
+  const unsigned who = __ballot_sync(~0u, has) >> (lane & ~3) & 15u;
+  top = __shfl_sync(~0u, mine, (lane & ~3) + (who ? __ffs(who) - 1 : 0));
+  const float d = __fdiv_rn(top, -8.f);
+  const float inv = d != 0.f ? __fdiv_rn(1.f, d) : 0.f;
   uint32_t word = 0;
-  float mine = 0.f;
 #pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    unsigned long long key = 0;
-#pragma unroll
-    for (int i = 0; i < PB; ++i) {
-      const uint32_t bits = __float_as_uint(x[b * PB + i]);
-      const unsigned long long c = ((unsigned long long)(bits & 0x7fffffffu) << 6) |
-                                   (unsigned)((31 - (i * W + w)) << 1) | (bits >> 31);
-      key = c > key ? c : key;
-    }
-#pragma unroll
-    for (int o = W / 2; o; o >>= 1) {
-      const unsigned long long c = __shfl_xor_sync(~0u, key, o, W);
-      key = c > key ? c : key;
-    }
-    const float top = __uint_as_float((uint32_t)(key >> 6) | ((uint32_t)(key & 1) << 31));
-    const float d = __fdiv_rn(top, -8.f);
-    const float inv = d != 0.f ? __fdiv_rn(1.f, d) : 0.f;
-#pragma unroll
-    for (int i = 0; i < PB; ++i) {
-      // the product and the sum are rounded one by one, as the rule says
-      const float y = __fadd_rn(__fmul_rn(x[b * PB + i], inv), 8.5f);
-      const int code = (int)fminf(fmaxf(y, 0.f), 15.f);
-      word |= (uint32_t)code << (4 * kv4_nib(b * PB + i));
-    }
-    if (w == b) mine = d;
+  for (int i = 0; i < 8; ++i) {
+    // the product and the sum are rounded one by one, as the rule says
+    const float y = __fadd_rn(__fmul_rn(x[i], inv), 8.5f);
+    word |= (uint32_t)(int)fminf(fmaxf(y, 0.f), 15.f) << (4 * i);
   }
-  if (slot < 0 || slot >= a.n_slots) return;
+  word = nibbles_out(nibble_transpose<D>(word));
+  if (!on) return;
   const int s = slot % kKv4Page;
   uint8_t* page = a.pool + ((size_t)(slot / kKv4Page) * a.Hk + h) * kv4_page_bytes(D);
-  ((uint32_t*)(page + kv * 32 * D + s * (D / 2)))[kv4_word_at<D>(s, w)] = word;
-  if (w < NB)
-    ((__half*)(page + 64 * D + kv * 4 * D))[kv4_scale_at(s, w, NB)] = __float2half_rn(mine);
+  ((uint32_t*)(page + kv * 32 * D + s * (D / 2)))[kv4_word_at<D>(s, lane_word<D>(c))] = word;
+  if (c % 4 == 0) ((__half*)(page + 64 * D + kv * 4 * D))[kv4_scale_at(s, c / 4, NB)] = __float2half_rn(d);
 }
 
 struct ReadArgs {
@@ -340,29 +381,32 @@ struct ReadArgs {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(256) k_kv4_read(const ReadArgs a) {
-  constexpr int W = D / 8, NB = D / 32, PB = 32 / W;
+  constexpr int W = D / 8, NB = D / 32, V = 16 / sizeof(T);
   const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / W;
-  const int w = threadIdx.x % W;
-  if (row >= 2ll * a.T * a.Hk) return;
-  const int kv = (int)(row % 2), h = (int)((row / 2) % a.Hk);
-  const long long t = row / 2 / a.Hk;
-  const int slot = a.slots[t];
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  const int c = threadIdx.x % W;
+  const bool live = row < 2ll * a.T * a.Hk;
+  const uint32_t th = live ? (uint32_t)(row / 2) : 0u;
+  const int kv = (int)(row & 1), h = (int)(th % (uint32_t)a.Hk);
+  const long long t = th / (uint32_t)a.Hk;
+  const int slot = live ? a.slots[t] : -1;
+  uint32_t word = 0;
+  float d = 0.f;
   if (slot >= 0 && slot < a.n_slots) {
     const int s = slot % kKv4Page;
     const uint8_t* page = a.pool + ((size_t)(slot / kKv4Page) * a.Hk + h) * kv4_page_bytes(D);
-    const uint32_t word = ((const uint32_t*)(page + kv * 32 * D + s * (D / 2)))[kv4_word_at<D>(s, w)];
-    const __half* sc = (const __half*)(page + 64 * D + kv * 4 * D);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      x[i] = (float)((int)((word >> (4 * kv4_nib(i))) & 15) - 8) *
-             __half2float(sc[kv4_scale_at(s, i / PB, NB)]);
+    word = ((const uint32_t*)(page + kv * 32 * D + s * (D / 2)))[kv4_word_at<D>(s, lane_word<D>(c))];
+    d = __half2float(((const __half*)(page + 64 * D + kv * 4 * D))[kv4_scale_at(s, c / 4, NB)]);
   }
-  T* o = (T*)(kv ? a.v : a.k) + (t * a.Hk + h) * D;
+  word = nibble_transpose<D>(nibbles_in(word));  // its own inverse
+  if (!live) return;
+  Pack<T, V>* o = (Pack<T, V>*)((T*)(kv ? a.v : a.k) + (t * a.Hk + h) * D + 8 * c);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) o[i * W + w] = from_f<T>(x[i]);
+  for (int k = 0; k < 8 / V; ++k) {
+    Pack<T, V> y;
+#pragma unroll
+    for (int i = 0; i < V; ++i) y.x[i] = from_f<T>((float)((int)((word >> (4 * (k * V + i))) & 15) - 8) * d);
+    o[k] = y;
+  }
 }
 
 template <template <typename, int> class F, int D, typename... A>
@@ -375,7 +419,11 @@ template <typename T, int D>
 struct Append {
   static cudaError_t run(const AppendArgs& a, cudaStream_t s) {
     const long long n = 2ll * a.T * a.Hk * (D / 8);
-    k_kv4_append<T, D><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a);
+    const unsigned grid = (unsigned)((n + 255) / 256);
+    // 16-byte loads where every row starts at a multiple of them
+    const long long any = (a.k_tok | a.k_head | a.v_tok | a.v_head) * (long long)sizeof(T);
+    if (any % 16 == 0 && aligned(a.k, 16) && aligned(a.v, 16)) k_kv4_append<T, D, true><<<grid, 256, 0, s>>>(a);
+    else k_kv4_append<T, D, false><<<grid, 256, 0, s>>>(a);
     return cudaGetLastError();
   }
 };
@@ -510,8 +558,8 @@ extern "C" mc_status mc_kv4_append(const mc_kv4_append_args* args, int32_t devic
   if (n_tokens < 0) return set_error(MC_E_INVALID, "negative size");
   if (n_tokens == 0) return MC_OK;
   if (!k || !v || !slots) return set_error(MC_E_INVALID, "null pointer");
-  if ((long long)n_tokens * n_kv_heads * head_dim / 4 >= (1ll << 39))
-    return set_error(MC_E_CAPACITY, "too many values for one call");
+  if ((long long)n_tokens * n_kv_heads > 0x7fffffffll)
+    return set_error(MC_E_CAPACITY, "too many rows for one call");
   MC_PCKS(paged_device(device));
   AppendArgs a{k, v, k_tok, k_head, v_tok, v_head, slots, (uint8_t*)pool, n_tokens, n_kv_heads,
                (int)(n_pages * kKv4Page)};
@@ -533,6 +581,10 @@ extern "C" mc_status mc_kv4_read(const mc_kv4_read_args* args, int32_t device, v
   if (n_tokens < 0) return set_error(MC_E_INVALID, "negative size");
   if (n_tokens == 0) return MC_OK;
   if (!k_out || !v_out || !slots) return set_error(MC_E_INVALID, "null pointer");
+  if (!aligned(k_out, 16) || !aligned(v_out, 16))
+    return set_error(MC_E_INVALID, "outputs must be 16-byte aligned");
+  if ((long long)n_tokens * n_kv_heads > 0x7fffffffll)
+    return set_error(MC_E_CAPACITY, "too many rows for one call");
   MC_PCKS(paged_device(device));
   ReadArgs a{(const uint8_t*)pool, slots, k_out, v_out, n_tokens, n_kv_heads, (int)(n_pages * kKv4Page)};
   MC_PCK(head_dim == 128 ? (by_type<Read, 128>(dtype, a, (cudaStream_t)stream))
