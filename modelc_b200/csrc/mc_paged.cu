@@ -310,34 +310,9 @@ __device__ __forceinline__ int lane_word(int c) {
   return D == 128 ? 8 * (c & 1) + (c >> 1) : c;
 }
 
-template <typename T, int D, bool VEC>
-__global__ void __launch_bounds__(256) k_kv4_append(const AppendArgs a) {
-  constexpr int W = D / 8, NB = D / 32;
-  const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / W;
-  const int c = threadIdx.x % W, lane = threadIdx.x & 31;
-  const bool live = row < 2ll * a.T * a.Hk;
-  const uint32_t th = live ? (uint32_t)(row / 2) : 0u;  // T Hk < 2^31
-  const int kv = (int)(row & 1), h = (int)(th % (uint32_t)a.Hk);
-  const long long t = th / (uint32_t)a.Hk;
-  const int slot = live ? a.slots[t] : -1;
-  const bool on = slot >= 0 && slot < a.n_slots;
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = 0.f;
-  if (on) {
-    const T* p = (kv ? (const T*)a.v + t * a.v_tok + h * a.v_head : (const T*)a.k + t * a.k_tok + h * a.k_head) + 8 * c;
-    if (VEC) {
-      const Pack<T, 16 / sizeof(T)>* v = (const Pack<T, 16 / sizeof(T)>*)p;
-      Pack<T, 16 / sizeof(T)> y[sizeof(T) / 2];
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) y[i] = v[i];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = to_f(y[i / (16 / sizeof(T))].x[i % (16 / sizeof(T))]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = to_f(p[i]);
-    }
-  }
+// The codes of 8 values x of one lane and their block's d.
+__device__ __forceinline__ uint32_t quantize8(const float (&x)[8], float& d) {
+  const int lane = threadIdx.x & 31;
   // the block's largest size over its 4 lanes (a NaN stays one), then the
   // first value that has it
   float top = fabsf(x[0]);
@@ -355,7 +330,7 @@ __global__ void __launch_bounds__(256) k_kv4_append(const AppendArgs a) {
     if (fabsf(x[i]) == top) mine = x[i], has = true;
   const unsigned who = __ballot_sync(~0u, has) >> (lane & ~3) & 15u;
   top = __shfl_sync(~0u, mine, (lane & ~3) + (who ? __ffs(who) - 1 : 0));
-  const float d = __fdiv_rn(top, -8.f);
+  d = __fdiv_rn(top, -8.f);
   const float inv = d != 0.f ? __fdiv_rn(1.f, d) : 0.f;
   uint32_t word = 0;
 #pragma unroll
@@ -364,12 +339,47 @@ __global__ void __launch_bounds__(256) k_kv4_append(const AppendArgs a) {
     const float y = __fadd_rn(__fmul_rn(x[i], inv), 8.5f);
     word |= (uint32_t)(int)fminf(fmaxf(y, 0.f), 15.f) << (4 * i);
   }
-  word = nibbles_out(nibble_transpose<D>(word));
-  if (!on) return;
-  const int s = slot % kKv4Page;
-  uint8_t* page = a.pool + ((size_t)(slot / kKv4Page) * a.Hk + h) * kv4_page_bytes(D);
-  ((uint32_t*)(page + kv * 32 * D + s * (D / 2)))[kv4_word_at<D>(s, lane_word<D>(c))] = word;
-  if (c % 4 == 0) ((__half*)(page + 64 * D + kv * 4 * D))[kv4_scale_at(s, c / 4, NB)] = __float2half_rn(d);
+  return word;
+}
+
+// A thread takes K and V of PER (token, head) pairs, `step` apart, and has
+// all their loads under way before it uses the first.
+template <typename T, int D, bool VEC, int PER>
+__global__ void __launch_bounds__(256) k_kv4_append(const AppendArgs a, uint32_t step) {
+  constexpr int W = D / 8, NB = D / 32, V = VEC ? 16 / sizeof(T) : 1, N = 8 / V;
+  const uint32_t first = (uint32_t)(((long long)blockIdx.x * 256 + threadIdx.x) / W), total = (uint32_t)(a.T * a.Hk);
+  const int c = threadIdx.x % W;
+  int slot[PER], h[PER];
+  Pack<T, V> y[PER][2][N];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const uint32_t th = first + i * step;
+    const bool live = first < step && th < total;
+    const uint32_t t = live ? th / (uint32_t)a.Hk : 0u;
+    h[i] = live ? (int)(th - t * (uint32_t)a.Hk) : 0;
+    slot[i] = live ? a.slots[t] : -1;
+    const T* k = (const T*)a.k + t * a.k_tok + h[i] * a.k_head + 8 * c;
+    const T* v = (const T*)a.v + t * a.v_tok + h[i] * a.v_head + 8 * c;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      y[i][0][n] = ((const Pack<T, V>*)k)[n];
+      y[i][1][n] = ((const Pack<T, V>*)v)[n];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      float x[8], d;
+#pragma unroll
+      for (int n = 0; n < 8; ++n) x[n] = to_f(y[i][kv][n / V].x[n % V]);
+      const uint32_t word = nibbles_out(nibble_transpose<D>(quantize8(x, d)));
+      if (slot[i] < 0 || slot[i] >= a.n_slots) continue;
+      const int s = slot[i] % kKv4Page;
+      uint8_t* page = a.pool + ((size_t)(slot[i] / kKv4Page) * a.Hk + h[i]) * kv4_page_bytes(D);
+      ((uint32_t*)(page + kv * 32 * D + s * (D / 2)))[kv4_word_at<D>(s, lane_word<D>(c))] = word;
+      if (c % 4 == 0) ((__half*)(page + 64 * D + kv * 4 * D))[kv4_scale_at(s, c / 4, NB)] = __float2half_rn(d);
+    }
 }
 
 struct ReadArgs {
@@ -379,34 +389,47 @@ struct ReadArgs {
   int T, Hk, n_slots;
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(256) k_kv4_read(const ReadArgs a) {
+template <typename T, int D, int PER>
+__global__ void __launch_bounds__(256) k_kv4_read(const ReadArgs a, uint32_t step) {
   constexpr int W = D / 8, NB = D / 32, V = 16 / sizeof(T);
-  const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / W;
+  const uint32_t first = (uint32_t)(((long long)blockIdx.x * 256 + threadIdx.x) / W), total = (uint32_t)(a.T * a.Hk);
   const int c = threadIdx.x % W;
-  const bool live = row < 2ll * a.T * a.Hk;
-  const uint32_t th = live ? (uint32_t)(row / 2) : 0u;
-  const int kv = (int)(row & 1), h = (int)(th % (uint32_t)a.Hk);
-  const long long t = th / (uint32_t)a.Hk;
-  const int slot = live ? a.slots[t] : -1;
-  uint32_t word = 0;
-  float d = 0.f;
-  if (slot >= 0 && slot < a.n_slots) {
-    const int s = slot % kKv4Page;
-    const uint8_t* page = a.pool + ((size_t)(slot / kKv4Page) * a.Hk + h) * kv4_page_bytes(D);
-    word = ((const uint32_t*)(page + kv * 32 * D + s * (D / 2)))[kv4_word_at<D>(s, lane_word<D>(c))];
-    d = __half2float(((const __half*)(page + 64 * D + kv * 4 * D))[kv4_scale_at(s, c / 4, NB)]);
-  }
-  word = nibble_transpose<D>(nibbles_in(word));  // its own inverse
-  if (!live) return;
-  Pack<T, V>* o = (Pack<T, V>*)((T*)(kv ? a.v : a.k) + (t * a.Hk + h) * D + 8 * c);
+  uint32_t word[PER][2] = {};
+  float d[PER][2] = {};
+  int slot[PER];
 #pragma unroll
-  for (int k = 0; k < 8 / V; ++k) {
-    Pack<T, V> y;
-#pragma unroll
-    for (int i = 0; i < V; ++i) y.x[i] = from_f<T>((float)((int)((word >> (4 * (k * V + i))) & 15) - 8) * d);
-    o[k] = y;
+  for (int i = 0; i < PER; ++i) {
+    const uint32_t th = first + i * step;
+    slot[i] = first < step && th < total ? a.slots[th / (uint32_t)a.Hk] : -1;
   }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (slot[i] < 0 || slot[i] >= a.n_slots) continue;
+    const int s = slot[i] % kKv4Page, h = (int)((first + i * step) % (uint32_t)a.Hk);
+    const uint8_t* page = a.pool + ((size_t)(slot[i] / kKv4Page) * a.Hk + h) * kv4_page_bytes(D);
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      word[i][kv] = ((const uint32_t*)(page + kv * 32 * D + s * (D / 2)))[kv4_word_at<D>(s, lane_word<D>(c))];
+      d[i][kv] = __half2float(((const __half*)(page + 64 * D + kv * 4 * D))[kv4_scale_at(s, c / 4, NB)]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      const uint32_t w = nibble_transpose<D>(nibbles_in(word[i][kv]));  // its own inverse
+      const uint32_t th = first + i * step;
+      if (first >= step || th >= total) continue;
+      Pack<T, V>* o = (Pack<T, V>*)((T*)(kv ? a.v : a.k) + (size_t)th * D + 8 * c);
+#pragma unroll
+      for (int k = 0; k < 8 / V; ++k) {
+        Pack<T, V> y;
+#pragma unroll
+        for (int n = 0; n < V; ++n)
+          y.x[n] = from_f<T>((float)((int)((w >> (4 * (k * V + n))) & 15) - 8) * d[i][kv]);
+        o[k] = y;
+      }
+    }
 }
 
 template <template <typename, int> class F, int D, typename... A>
@@ -415,23 +438,43 @@ static cudaError_t by_type(int dtype, A&&... args) {
   if (dtype == MC_ACT_F16) return F<__half, D>::run(args...);
   return F<__nv_bfloat16, D>::run(args...);
 }
+// (token, head) pairs that one thread takes: two once the single ones would
+// fill the GPU more than once.
+template <int D>
+static int rows_per(int device, long long pairs) {
+  return pairs * (D / 8) > 2048ll * paged_sms(device) ? 2 : 1;
+}
+static unsigned row_grid(uint32_t step, int W) { return (unsigned)(((long long)step * W + 255) / 256); }
 template <typename T, int D>
 struct Append {
-  static cudaError_t run(const AppendArgs& a, cudaStream_t s) {
-    const long long n = 2ll * a.T * a.Hk * (D / 8);
-    const unsigned grid = (unsigned)((n + 255) / 256);
+  template <bool VEC>
+  static cudaError_t run_vec(const AppendArgs& a, int device, cudaStream_t s) {
+    const uint32_t n = (uint32_t)(a.T * a.Hk);
+    if (rows_per<D>(device, n) == 2) {
+      const uint32_t step = (n + 1) / 2;
+      k_kv4_append<T, D, VEC, 2><<<row_grid(step, D / 8), 256, 0, s>>>(a, step);
+    } else {
+      k_kv4_append<T, D, VEC, 1><<<row_grid(n, D / 8), 256, 0, s>>>(a, n);
+    }
+    return cudaGetLastError();
+  }
+  static cudaError_t run(const AppendArgs& a, int device, cudaStream_t s) {
     // 16-byte loads where every row starts at a multiple of them
     const long long any = (a.k_tok | a.k_head | a.v_tok | a.v_head) * (long long)sizeof(T);
-    if (any % 16 == 0 && aligned(a.k, 16) && aligned(a.v, 16)) k_kv4_append<T, D, true><<<grid, 256, 0, s>>>(a);
-    else k_kv4_append<T, D, false><<<grid, 256, 0, s>>>(a);
-    return cudaGetLastError();
+    return any % 16 == 0 && aligned(a.k, 16) && aligned(a.v, 16) ? run_vec<true>(a, device, s)
+                                                                  : run_vec<false>(a, device, s);
   }
 };
 template <typename T, int D>
 struct Read {
-  static cudaError_t run(const ReadArgs& a, cudaStream_t s) {
-    const long long n = 2ll * a.T * a.Hk * (D / 8);
-    k_kv4_read<T, D><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a);
+  static cudaError_t run(const ReadArgs& a, int device, cudaStream_t s) {
+    const uint32_t n = (uint32_t)(a.T * a.Hk);
+    if (rows_per<D>(device, n) == 2) {
+      const uint32_t step = (n + 1) / 2;
+      k_kv4_read<T, D, 2><<<row_grid(step, D / 8), 256, 0, s>>>(a, step);
+    } else {
+      k_kv4_read<T, D, 1><<<row_grid(n, D / 8), 256, 0, s>>>(a, n);
+    }
     return cudaGetLastError();
   }
 };
@@ -563,8 +606,8 @@ extern "C" mc_status mc_kv4_append(const mc_kv4_append_args* args, int32_t devic
   MC_PCKS(paged_device(device));
   AppendArgs a{k, v, k_tok, k_head, v_tok, v_head, slots, (uint8_t*)pool, n_tokens, n_kv_heads,
                (int)(n_pages * kKv4Page)};
-  MC_PCK(head_dim == 128 ? (by_type<Append, 128>(dtype, a, (cudaStream_t)stream))
-                         : (by_type<Append, 64>(dtype, a, (cudaStream_t)stream)));
+  MC_PCK(head_dim == 128 ? (by_type<Append, 128>(dtype, a, device, (cudaStream_t)stream))
+                         : (by_type<Append, 64>(dtype, a, device, (cudaStream_t)stream)));
   return MC_OK;
 }
 
@@ -587,7 +630,7 @@ extern "C" mc_status mc_kv4_read(const mc_kv4_read_args* args, int32_t device, v
     return set_error(MC_E_CAPACITY, "too many rows for one call");
   MC_PCKS(paged_device(device));
   ReadArgs a{(const uint8_t*)pool, slots, k_out, v_out, n_tokens, n_kv_heads, (int)(n_pages * kKv4Page)};
-  MC_PCK(head_dim == 128 ? (by_type<Read, 128>(dtype, a, (cudaStream_t)stream))
-                         : (by_type<Read, 64>(dtype, a, (cudaStream_t)stream)));
+  MC_PCK(head_dim == 128 ? (by_type<Read, 128>(dtype, a, device, (cudaStream_t)stream))
+                         : (by_type<Read, 64>(dtype, a, device, (cudaStream_t)stream)));
   return MC_OK;
 }
