@@ -596,84 +596,83 @@ __global__ void __launch_bounds__(32 * kKv4Warps<NP>, 1) k_kv4(const Kv4Args a) 
 
 // Joins the parts of the rows that several warps worked on, in the line's
 // order whatever the order in which they came; zeroes rows of no request.
-// One block a row: the request in one round of loads, the weights of the
-// parts in a second, their sums in a third.
-constexpr int kJoinThreads = 256;
+// One block for a token's rows of one key/value head: the request in one
+// round of loads, the maximum over a row's parts in a second, their sums in a
+// third, kJoinWarps / group warps to a row.  (One block a row, 2048 of them for
+// 32 requests of 64 heads, took 10 us where this takes 5.)
+constexpr int kJoinWarps = 16;
 template <typename T, int D, int NP>
-__global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const Kv4Args a) {
-  constexpr int R = 8 * NP, V = D / 32, kWarps = kJoinThreads / 32;
-  constexpr int kParts = 1024;  // parts whose weights are kept at a time
-  __shared__ float s_w[kParts], s_o[kWarps][D], s_red[2 * kWarps];
+__global__ void __launch_bounds__(32 * kJoinWarps) k_kv4_join(const Kv4Args a) {
+  constexpr int R = 8 * NP, V = D / 32;
+  __shared__ float s_o[kJoinWarps][D], s_l[kJoinWarps];
+  __shared__ Kv4Req s_rq;
   __shared__ long long s_first;
-  __shared__ int s_req[4];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  const int row = blockIdx.x, t = row / a.H, h = row - t * a.H, G = a.H / a.Hk, hk = h / G;
-  if (tid == 0) s_req[0] = 0;
+  const int t = blockIdx.x / a.Hk, hk = blockIdx.x - t * a.Hk, G = a.H / a.Hk;
+  if (tid == 0) s_rq.n = 0;
   __syncthreads();
   grid_wait();
   const long long L = __ldcg(a.head), N = __ldcg(a.head + 1);
-  for (int z = tid; z < a.B; z += kJoinThreads) {
+  for (int z = tid; z < a.B; z += 32 * kJoinWarps) {
     const Kv4Req rq = kv4_req<R>(a, z);
     const long long first = __ldcg(a.head + 2 + z);
-    if (rq.c0 <= t && t < rq.c0 + rq.n) {
-      const int idx = (t - rq.c0) * G + (h - hk * G), rb = idx / R;
-      s_req[0] = rq.pages, s_req[1] = idx - rb * R;
-      s_first = first + ((long long)hk * rq.nb + rb) * rq.pages;
-    }
+    if (rq.c0 <= t && t < rq.c0 + rq.n) s_rq = rq, s_first = first;
   }
   __syncthreads();
-  T* out = (T*)a.out + (size_t)row * D;
-  if (!s_req[0]) {
-    for (int d = tid; d < D; d += kJoinThreads) out[d] = from_f<T>(0.f);
+  const Kv4Req rq = s_rq;
+  T* out = (T*)a.out + ((size_t)t * a.H + (size_t)hk * G) * D;
+  if (!rq.n) {
+    for (int d = tid; d < G * D; d += 32 * kJoinWarps) out[d] = from_f<T>(0.f);
     return;
   }
-  const int r = s_req[1];
-  const long long s0 = s_first;
-  const int w0 = (int)(((s0 + 1) * N - 1) / L), w1 = (int)(((s0 + s_req[0]) * N - 1) / L), n = w1 - w0 + 1;
-  if (n == 1) return;  // written by its warp
-  // only the first part can be its warp's second row block
-  const int slot0 = 2 * w0 + ((long long)w0 * L / N >= s0 ? 0 : 1);
-  auto at = [&](int i) { return (size_t)(i ? 2 * (w0 + i) : slot0) * R + r; };
-  float top = -INFINITY, sum = 0.f, o[V] = {};
-  for (int i = tid; i < n; i += kJoinThreads) top = fmaxf(top, __ldcg(a.ml + 2 * at(i)));
+  const int per = max(1, kJoinWarps / G), at_once = kJoinWarps / per;  // warps to a row, rows at once
+  const int sub = wid % per;
+  for (int r0 = 0; r0 < G; r0 += at_once) {
+    const int r = r0 + wid / per;
+    int n = 0;
+    float o[V] = {}, l = 0.f;
+    if (wid / per < at_once && r < G) {
+      const int idx = (t - rq.c0) * G + r, rb = idx / R, row = idx - rb * R;
+      const long long s0 = s_first + ((long long)hk * rq.nb + rb) * rq.pages;
+      const int w0 = (int)(((s0 + 1) * N - 1) / L);
+      n = (int)(((s0 + rq.pages) * N - 1) / L) - w0 + 1;
+      // only the first part can be its warp's second row block
+      const int slot0 = 2 * w0 + ((long long)w0 * L / N >= s0 ? 0 : 1);
+      auto at = [&](int i) { return (size_t)(i ? 2 * (w0 + i) : slot0) * R + row; };
+      if (n > 1) {  // one part was written by its warp
+        float top = -INFINITY;
+        for (int i = lane; i < n; i += 32) top = fmaxf(top, __ldcg(a.ml + 2 * at(i)));
 #pragma unroll
-  for (int f = 16; f; f >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, f));
-  if (lane == 0) s_red[wid] = top;
-  __syncthreads();
+        for (int f = 16; f; f >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, f));
+#pragma unroll 4
+        for (int i = sub; i < n; i += per) {
+          const float2 ml = __ldcg((const float2*)(a.ml + 2 * at(i)));
+          float x[V];
+          if constexpr (V == 4) *(float4*)x = __ldcg((const float4*)(a.part + at(i) * D) + lane);
+          else *(float2*)x = __ldcg((const float2*)(a.part + at(i) * D) + lane);
+          // a part without keys has no sum, unless its copies failed
+          const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+          l += ml.y != ml.y ? ml.y : f * ml.y;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_red[w]);
-  for (int i0 = 0; i0 < n; i0 += kParts) {
-    const int cnt = min(kParts, n - i0);
-    if (i0) __syncthreads();
-    for (int i = tid; i < cnt; i += kJoinThreads) {
-      const float2 ml = __ldcg((const float2*)(a.ml + 2 * at(i0 + i)));
-      // a part without keys has no sum, unless its copies failed
-      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
-      s_w[i] = f;
-      sum += ml.y != ml.y ? ml.y : f * ml.y;
+          for (int v = 0; v < V; ++v) o[v] += f == 0.f ? 0.f : f * x[v];
+        }
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) s_o[wid][lane * V + v] = o[v];
+    if (lane == 0) s_l[wid] = l;
+    __syncthreads();
+    if (n > 1 && sub == 0) {
+      float all = 0.f, y[V] = {};
+      for (int w = 0; w < per; ++w) {
+        all += s_l[wid + w];
+#pragma unroll
+        for (int v = 0; v < V; ++v) y[v] += s_o[wid + w][lane * V + v];
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) out[r * D + lane * V + v] = from_f<T>(all != 0.f ? y[v] / all : 0.f);
     }
     __syncthreads();
-#pragma unroll 4
-    for (int i = wid; i < cnt; i += kWarps) {
-      const float f = s_w[i];
-      float x[V];
-      if constexpr (V == 4) *(float4*)x = __ldcg((const float4*)(a.part + at(i0 + i) * D) + lane);
-      else *(float2*)x = __ldcg((const float2*)(a.part + at(i0 + i) * D) + lane);
-#pragma unroll
-      for (int v = 0; v < V; ++v) o[v] += f == 0.f ? 0.f : f * x[v];
-    }
-  }
-#pragma unroll
-  for (int f = 16; f; f >>= 1) sum += __shfl_xor_sync(~0u, sum, f);
-  if (lane == 0) s_red[kWarps + wid] = sum;
-#pragma unroll
-  for (int v = 0; v < V; ++v) s_o[wid][lane * V + v] = o[v];
-  __syncthreads();
-  if (tid < D) {
-    float y = 0.f, all = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) y += s_o[w][tid], all += s_red[kWarps + w];
-    out[tid] = from_f<T>(all != 0.f ? y / all : 0.f);
   }
 }
 
@@ -689,11 +688,13 @@ static Kv4Space kv4_space(int sms, int B, int rows, int D) {
   s.total = s.part + slots * rows * D * 4;
   return s;
 }
-// Query rows of a block: the fewest of 8, 16, 24 that hold a request's rows
-// (tokens times grouped heads) on average.
+// Query rows of a block: 16 where a request has more rows (tokens times
+// grouped heads) than that on average, else 8, with the twelve warps that its
+// registers allow.  Blocks of 8, which dequantize a page once for each 8 rows,
+// against 16, at D = 128: 105 and 119 us for 24 requests of 12 rows on
+// average, 229 and 203 us for 36 rows.  Blocks of 24 lost to both.
 static int kv4_rows(int T, int B, int H, int Hk) {
-  const long long rows = (long long)T * (H / Hk), b = std::max(B, 1);
-  return rows <= 8 * b ? 8 : rows <= 16 * b ? 16 : 24;
+  return (long long)T * (H / Hk) <= 16ll * std::max(B, 1) ? 8 : 16;
 }
 
 template <typename T, int D, int NP>
@@ -715,8 +716,8 @@ static cudaError_t run_kv4(const Kv4Args& a, int sms, cudaStream_t s) {
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)(a.T * a.H));
-  cfg.blockDim = dim3(kJoinThreads);
+  cfg.gridDim = dim3((unsigned)(a.T * a.Hk));
+  cfg.blockDim = dim3(32 * kJoinWarps);
   cfg.stream = s;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
@@ -724,9 +725,7 @@ static cudaError_t run_kv4(const Kv4Args& a, int sms, cudaStream_t s) {
 }
 template <typename T, int D>
 static cudaError_t run_kv4_rows(const Kv4Args& a, int rows, int sms, cudaStream_t s) {
-  return rows == 8    ? run_kv4<T, D, 1>(a, sms, s)
-         : rows == 16 ? run_kv4<T, D, 2>(a, sms, s)
-                      : run_kv4<T, D, 3>(a, sms, s);
+  return rows == 8 ? run_kv4<T, D, 1>(a, sms, s) : run_kv4<T, D, 2>(a, sms, s);
 }
 
 }  // namespace mc
@@ -738,7 +737,7 @@ extern "C" int64_t mc_kv4_attention_workspace(int32_t n_requests, int32_t head_d
   if (paged_device(device) != MC_OK) return 0;
   const int sms = paged_sms(device);
   return (int64_t)std::max(kv4_space(sms, n_requests, 8, head_dim).total,
-                           kv4_space(sms, n_requests, 24, head_dim).total);
+                           kv4_space(sms, n_requests, 16, head_dim).total);
 }
 
 extern "C" mc_status mc_kv4_attention(const mc_kv4_attention_args* args, int32_t device, void* stream) {
