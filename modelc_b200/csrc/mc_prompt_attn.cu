@@ -162,28 +162,20 @@ struct PromptWork {
 // first, since under a causal mask they have the most keys.  One warp.
 __device__ __forceinline__ void prompt_work(const PromptArgs& a, int index, PromptWork* w) {
   const int lane = threadIdx.x & 31;
-  int total = 0;
-  for (int z0 = 0; z0 < a.B; z0 += 32) {
-    const int z = z0 + lane;
-    int n = 0;
-    if (z < a.B) {
-      const int c0 = min(max(a.cu_q[z], 0), a.Tq);
-      n = max(min(a.cu_q[z + 1], a.Tq) - c0, 0);
-    }
-    total += __reduce_add_sync(~0u, (n + a.rows - 1) / a.rows);
-  }
+  // the sequences from the last one down, 32 at a time; all four bounds are
+  // read at once, since this load's latency is most of a short block's start
+  int seen = 0;
   if (lane == 0) w->ok = 0;
   __syncwarp();
-  const int want = total - 1 - index;
-  if (want < 0) return;
-  int seen = 0;
-  for (int z0 = 0; z0 < a.B; z0 += 32) {
-    const int z = z0 + lane;
-    int n = 0, c0 = 0;
-    if (z < a.B) {
-      c0 = min(max(a.cu_q[z], 0), a.Tq);
-      n = max(min(a.cu_q[z + 1], a.Tq) - c0, 0);
-    }
+  for (int z1 = a.B; z1 > 0 && seen <= index; z1 -= 32) {
+    const int z = z1 - 1 - lane;
+    int c0 = 0, n = 0, k0 = 0, k1 = 0;
+    if (z >= 0) c0 = a.cu_q[z], n = a.cu_q[z + 1], k0 = a.cu_k[z], k1 = a.cu_k[z + 1];
+    const int keys = k1 - k0;
+    c0 = min(max(c0, 0), a.Tq);
+    n = max(min(n, a.Tq) - c0, 0);
+    k0 = min(max(k0, 0), a.Tk);
+    k1 = max(min(k1, a.Tk), k0);
     const int mine = (n + a.rows - 1) / a.rows;
     int inc = mine;
 #pragma unroll
@@ -191,19 +183,17 @@ __device__ __forceinline__ void prompt_work(const PromptArgs& a, int index, Prom
       const int x = __shfl_up_sync(~0u, inc, o);
       if (lane >= o) inc += x;
     }
-    const int first = seen + inc - mine;
-    if (want >= first && want < first + mine) {
-      const int r = (want - first) * a.rows;
-      const int k0 = min(max(a.cu_k[z], 0), a.Tk), k1 = max(min(a.cu_k[z + 1], a.Tk), k0);
+    const int last = seen + inc - 1;  // the sequence's tiles are last - mine + 1 .. last, its last tile first
+    if (index <= last && index > last - mine) {
+      const int r = (last - index) * a.rows;
       w->q0 = c0 + r;
       w->n_q = n - r;
       w->k0 = k0;
       w->L = k1 - k0;
-      w->shift = a.causal ? (a.cu_k[z + 1] - a.cu_k[z]) - n + r + 1 : 1 << 30;
+      w->shift = a.causal ? keys - n + r + 1 : 1 << 30;
       w->ok = 1;
     }
     seen += __shfl_sync(~0u, inc, 31);
-    if (seen > want) break;
   }
   __syncwarp();
 }
@@ -267,16 +257,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   // tile t has the rows from t * row_1 of head + t * pair
   const int head = a.pair ? 2 * unit : unit, row_1 = a.pair ? 0 : kPromptRows;
 
-  // rows of no sequence are 0: each block clears its share
-  {
-    const int end = min(max(a.B ? a.cu_q[a.B] : 0, 0), a.Tq);
-    const long long n = (long long)(a.Tq - end) * a.H * (D / 8);
-    uint4* z = (uint4*)((T*)a.out + (size_t)end * a.H * D);
-    for (long long i = (long long)blockIdx.x * kPromptThreads + tid; i < n; i += (long long)gridDim.x * kPromptThreads)
-      z[i] = make_uint4(0, 0, 0, 0);
-  }
-  if (warp == 0) prompt_work(a, index, &s_work);
-  if (tid == 32) {
+  // the start, spread over warps: the work, the barriers, tensor memory (this
+  // block is alone on its SM), and clearing the rows of no sequence
+  if (warp == 0) {
+    prompt_work(a, index, &s_work);
+  } else if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm_ptr(&s_tmem)), "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else if (tid == 32) {
     for (int i = 0; i < C::Slots; ++i) bar_init(&b_full[i], 1);
     for (int i = 0; i < kPromptRounds; ++i) bar_init(&b_round[i], 1);
     for (int i = 0; i < 2; ++i) {
@@ -286,17 +275,25 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     bar_init(&b_tail, 1), bar_init(&b_fix, 1);
     s_fail = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  __syncthreads();
-  if (!s_work.ok) return;
-  if (warp == 8) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm_ptr(&s_tmem)), "r"(512u)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else if (tid == 288) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mq) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
+  } else if (warp >= 10) {
+    const int end = min(max(a.cu_q[a.B], 0), a.Tq);
+    const long long n = (long long)(a.Tq - end) * a.H * (D / 8);
+    uint4* z = (uint4*)((T*)a.out + (size_t)end * a.H * D);
+    for (long long i = (long long)blockIdx.x * 64 + tid - 320; i < n; i += (long long)gridDim.x * 64)
+      z[i] = make_uint4(0, 0, 0, 0);
   }
   tm_before();
   __syncthreads();
   tm_after();
+  if (!s_work.ok) {
+    if (warp == 8)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s_tmem), "r"(512u) : "memory");
+    return;
+  }
   const uint32_t tmem = s_tmem;
   const PromptWork w = s_work;
   const int hk = head / (a.H / a.Hk);
