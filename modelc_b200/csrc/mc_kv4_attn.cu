@@ -37,7 +37,10 @@ namespace mc {
 
 // Warps of a block (one block fills an SM) and the shared memory that their
 // rings share: 12 warps of 2 pages of D = 128 (4 of D = 64) for 8 query rows,
-// 8 warps of 3 (6) for more rows, whose accumulators take the registers.
+// 8 warps of 3 (6) for 16 rows, whose accumulators take the registers.  (16
+// warps of 128 registers, two to a ring and each on half of every page, were
+// slower, 88 against 78 us for 273 MB: what bounds the kernel is the issue of
+// logic and f16 instructions, two cycles each, not their latency.)
 template <int NP>
 constexpr int kKv4Warps = NP == 1 ? 12 : 8;
 constexpr int kKv4Rings = 24 * kv4_page_bytes(128);
@@ -425,7 +428,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps<NP>, 1) k_kv4(const Kv4Args a) 
               if (base + 16 * c + k_row[e / 2] >= vis[p][1]) w.y = 0.f;
             }
             s[c][p][e] = w.x, s[c][p][e + 1] = w.y;
-            l[p].x += w.x, l[p].y += w.y;
+            l[p] = add2(l[p], w);
           }
       }
       // --- values, 16 tokens at a time
@@ -518,12 +521,13 @@ __global__ void __launch_bounds__(32 * kKv4Warps<NP>, 1) k_kv4(const Kv4Args a) 
       if (!failed && !warp_wait(&s_full[wid][st], phase)) failed = true;
       if (!failed && s_there[wid][st]) {
         const uint8_t* pg = ring + st * PB;
+        const int base = page * kKv4Page;
+        if (base + 64 <= first) {
+          step(pg, pg + 64 * D, base, std::false_type());
+          step(pg + 16 * D, pg + 66 * D, base + 32, std::false_type());
+        } else {
 #pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          const uint8_t *kp = pg + h * 16 * D, *sp = pg + 64 * D + h * 2 * D;
-          const int base = page * kKv4Page + 32 * h;
-          if (base + 32 <= first) step(kp, sp, base, std::false_type());
-          else step(kp, sp, base, std::true_type());
+          for (int h = 0; h < 2; ++h) step(pg + h * 16 * D, pg + 64 * D + h * 2 * D, base + 32 * h, std::true_type());
         }
       }
       __syncwarp();
