@@ -85,6 +85,21 @@ struct Kv4Place {
   int pages, nb;        // of the request: pages, row blocks
 };
 
+// a / b, rounded down: an f32 estimate, put right by whole products (a 64-bit
+// division takes a thousand cycles, and several stood between a warp and its
+// first page).  The estimate is off by a 2^-22 of the quotient, and by one.
+__device__ __forceinline__ long long line_div(long long a, long long b) {
+  long long q = (long long)((float)a * __frcp_rn((float)b));
+  while (q * b > a) --q;
+  while ((q + 1) * b <= a) ++q;
+  return q;
+}
+// First unit of warp w's stretch of a line of L units for N warps.
+__device__ __forceinline__ long long line_at(int w, long long L, long long N) {
+  const long long q = line_div(L, N);  // whole units for each, the rest spread
+  return q * w + line_div((L - q * N) * w, N);
+}
+
 // m16n8k16, f16 operands, f32 accumulators: d = a b + c
 __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                       uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
@@ -178,7 +193,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps<NP>, 1) k_kv4(const Kv4Args a) 
   if (me >= N) return;
   {
     // --- where the stretch starts
-    const long long u0 = me * L / N, u1 = (me + 1) * L / N;
+    const long long u0 = line_at(me, L, N), u1 = line_at(me + 1, L, N);
     int l = 0, r = kThreads;
     while (r - l > 1) {
       const int m = (l + r) >> 1;
@@ -600,15 +615,13 @@ __global__ void __launch_bounds__(32 * kKv4Warps<NP>, 1) k_kv4(const Kv4Args a) 
 
 // Joins the parts of the rows that several warps worked on, in the line's
 // order whatever the order in which they came; zeroes rows of no request.
-// One block for a token's rows of one key/value head: the request in one
-// round of loads, the maximum over a row's parts in a second, their sums in a
-// third, kJoinWarps / group warps to a row.  (One block a row, 2048 of them for
-// 32 requests of 64 heads, took 10 us where this takes 5.)
+// One block for a token's rows of one key/value head, kJoinWarps / group warps
+// to a row: the request in one round of loads, the parts in a second.
 constexpr int kJoinWarps = 16;
 template <typename T, int D, int NP>
 __global__ void __launch_bounds__(32 * kJoinWarps) k_kv4_join(const Kv4Args a) {
   constexpr int R = 8 * NP, V = D / 32;
-  __shared__ float s_o[kJoinWarps][D], s_l[kJoinWarps];
+  __shared__ float s_o[kJoinWarps][D], s_l[kJoinWarps], s_m[kJoinWarps];
   __shared__ Kv4Req s_rq;
   __shared__ long long s_first;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
@@ -634,47 +647,71 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_kv4_join(const Kv4Args a) {
   for (int r0 = 0; r0 < G; r0 += at_once) {
     const int r = r0 + wid / per;
     int n = 0;
-    float o[V] = {}, l = 0.f;
+    float o[V] = {}, l = 0.f, m = -INFINITY;
     if (wid / per < at_once && r < G) {
       const int idx = (t - rq.c0) * G + r, rb = idx / R, row = idx - rb * R;
       const long long s0 = s_first + ((long long)hk * rq.nb + rb) * rq.pages;
-      const int w0 = (int)(((s0 + 1) * N - 1) / L);
-      n = (int)(((s0 + rq.pages) * N - 1) / L) - w0 + 1;
+      // the warps whose stretches hold the row block's first and last unit
+      const int w0 = (int)line_div((s0 + 1) * N - 1, L);
+      n = (int)line_div((s0 + rq.pages) * N - 1, L) - w0 + 1;
       // only the first part can be its warp's second row block
-      const int slot0 = 2 * w0 + ((long long)w0 * L / N >= s0 ? 0 : 1);
-      auto at = [&](int i) { return (size_t)(i ? 2 * (w0 + i) : slot0) * R + row; };
+      const int second = (long long)w0 * L >= s0 * N ? 0 : 1;
+      auto at = [&](int i) { return (size_t)(2 * (w0 + i) + (i ? 0 : second)) * R + row; };
       if (n > 1) {  // one part was written by its warp
-        float top = -INFINITY;
-        for (int i = lane; i < n; i += 32) top = fmaxf(top, __ldcg(a.ml + 2 * at(i)));
+        constexpr int kBatch = 4;  // parts whose loads are under way at once
+#pragma unroll 1
+        for (int i0 = sub; i0 < n; i0 += kBatch * per) {
+          float2 ml[kBatch];
+          float x[kBatch][V];
 #pragma unroll
-        for (int f = 16; f; f >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, f));
-#pragma unroll 4
-        for (int i = sub; i < n; i += per) {
-          const float2 ml = __ldcg((const float2*)(a.ml + 2 * at(i)));
-          float x[V];
-          if constexpr (V == 4) *(float4*)x = __ldcg((const float4*)(a.part + at(i) * D) + lane);
-          else *(float2*)x = __ldcg((const float2*)(a.part + at(i) * D) + lane);
-          // a part without keys has no sum, unless its copies failed
-          const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
-          l += ml.y != ml.y ? ml.y : f * ml.y;
+          for (int k = 0; k < kBatch; ++k) {
+            const int i = i0 + k * per;
+            ml[k] = make_float2(-INFINITY, 0.f);
+            if (i < n) {
+              const size_t slot = at(i);
+              ml[k] = __ldcg((const float2*)(a.ml + slot * 2));
+              if constexpr (V == 4) *(float4*)x[k] = __ldcg((const float4*)(a.part + slot * D) + lane);
+              else *(float2*)x[k] = __ldcg((const float2*)(a.part + slot * D) + lane);
+            }
+          }
+          float top = m;
 #pragma unroll
-          for (int v = 0; v < V; ++v) o[v] += f == 0.f ? 0.f : f * x[v];
+          for (int k = 0; k < kBatch; ++k) top = fmaxf(top, ml[k].x);
+          const float f0 = m == -INFINITY ? 0.f : ex2(m - top);
+          m = top;
+          l *= f0;
+#pragma unroll
+          for (int v = 0; v < V; ++v) o[v] *= f0;
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k) {
+            // a part without keys has no sum, unless its copies failed
+            const float f = ml[k].x == -INFINITY ? 0.f : ex2(ml[k].x - top);
+            l += ml[k].y != ml[k].y ? ml[k].y : f * ml[k].y;
+#pragma unroll
+            for (int v = 0; v < V; ++v) o[v] += f == 0.f ? 0.f : f * x[k][v];
+          }
         }
       }
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) s_o[wid][lane * V + v] = o[v];
-    if (lane == 0) s_l[wid] = l;
+    if (lane == 0) s_l[wid] = l, s_m[wid] = m;
     __syncthreads();
     if (n > 1 && sub == 0) {
-      float all = 0.f, y[V] = {};
+      float all = 0.f, y[V] = {}, top = -INFINITY;
+#pragma unroll 1
+      for (int w = 0; w < per; ++w) top = fmaxf(top, s_m[wid + w]);
+#pragma unroll 1
       for (int w = 0; w < per; ++w) {
-        all += s_l[wid + w];
+        const float f = s_m[wid + w] == -INFINITY ? 0.f : ex2(s_m[wid + w] - top), lw = s_l[wid + w];
+        all += lw != lw ? lw : f * lw;
 #pragma unroll
-        for (int v = 0; v < V; ++v) y[v] += s_o[wid + w][lane * V + v];
+        for (int v = 0; v < V; ++v) y[v] += f == 0.f ? 0.f : f * s_o[wid + w][lane * V + v];
       }
 #pragma unroll
-      for (int v = 0; v < V; ++v) out[r * D + lane * V + v] = from_f<T>(all != 0.f ? y[v] / all : 0.f);
+      for (int v = 0; v < V; ++v) y[v] = all != 0.f ? y[v] / all : 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) out[r * D + lane * V + v] = from_f<T>(y[v]);
     }
     __syncthreads();
   }
