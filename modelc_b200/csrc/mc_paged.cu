@@ -332,14 +332,16 @@ __device__ __forceinline__ uint32_t quantize8(const float (&x)[8], float& d) {
   top = __shfl_sync(~0u, mine, (lane & ~3) + (who ? __ffs(who) - 1 : 0));
   d = __fdiv_rn(top, -8.f);
   const float inv = d != 0.f ? __fdiv_rn(1.f, d) : 0.f;
+  // codes without conversions: 2^23 + y, rounded down, has the code in its last
+  // bits, and what stands before them is taken off the word at once
   uint32_t word = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     // the product and the sum are rounded one by one, as the rule says
     const float y = __fadd_rn(__fmul_rn(x[i], inv), 8.5f);
-    word |= (uint32_t)(int)fminf(fmaxf(y, 0.f), 15.f) << (4 * i);
+    word += __float_as_uint(__fadd_rd(fminf(fmaxf(y, 0.f), 15.f), 8388608.f)) << (4 * i);
   }
-  return word;
+  return word - 0x4B000000u * 0x11111111u;
 }
 
 // A thread takes K and V of PER (token, head) pairs, `step` apart, and has
@@ -426,7 +428,8 @@ __global__ void __launch_bounds__(256) k_kv4_read(const ReadArgs a, uint32_t ste
         Pack<T, V> y;
 #pragma unroll
         for (int n = 0; n < V; ++n)
-          y.x[n] = from_f<T>((float)((int)((w >> (4 * (k * V + n))) & 15) - 8) * d[i][kv]);
+          // 2^23 + code, less 2^23 + 8
+          y.x[n] = from_f<T>((__uint_as_float(0x4B000000u | ((w >> (4 * (k * V + n))) & 15)) - 8388616.f) * d[i][kv]);
         o[k] = y;
       }
     }
