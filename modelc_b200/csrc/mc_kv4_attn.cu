@@ -624,16 +624,21 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_kv4_join(const Kv4Args a) {
   __shared__ float s_o[kJoinWarps][D], s_l[kJoinWarps], s_m[kJoinWarps];
   __shared__ Kv4Req s_rq;
   __shared__ long long s_first;
+  __shared__ int s_z;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int t = blockIdx.x / a.Hk, hk = blockIdx.x - t * a.Hk, G = a.H / a.Hk;
-  if (tid == 0) s_rq.n = 0;
+  if (tid == 0) s_rq.n = 0, s_z = a.B;
   __syncthreads();
   grid_wait();
   const long long L = __ldcg(a.head), N = __ldcg(a.head + 1);
-  for (int z = tid; z < a.B; z += 32 * kJoinWarps) {
-    const Kv4Req rq = kv4_req<R>(a, z);
-    const long long first = __ldcg(a.head + 2 + z);
-    if (rq.c0 <= t && t < rq.c0 + rq.n) s_rq = rq, s_first = first;
+  for (int z0 = 0; z0 < a.B; z0 += 32 * kJoinWarps) {
+    const int z = z0 + tid;
+    const Kv4Req rq = z < a.B ? kv4_req<R>(a, z) : Kv4Req{0, 0, 0, 0, 0};
+    const long long first = z < a.B ? __ldcg(a.head + 2 + z) : 0;
+    const bool mine = rq.c0 <= t && t < rq.c0 + rq.n;
+    if (mine) atomicMin(&s_z, z);  // should several claim the row, the first has it
+    __syncthreads();
+    if (mine && s_z == z) s_rq = rq, s_first = first;
   }
   __syncthreads();
   const Kv4Req rq = s_rq;

@@ -123,7 +123,8 @@ __global__ void __launch_bounds__(kSlotThreads) k_paged_slots(const SlotArgs a) 
         }
       }
       a.positions[t] = pos;
-      a.slots[t] = page < 0 ? -1 : page * a.page + pos % a.page;
+      const long long slot = (long long)page * a.page + pos % a.page;
+      a.slots[t] = page < 0 || slot > 0x7fffffffll ? -1 : (int)slot;
     }
     base_tok += n_tok;
     base_pg += n_pg;

@@ -280,11 +280,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
   } else if (warp >= 10) {
-    const int end = min(max(a.cu_q[a.B], 0), a.Tq);
-    const long long n = (long long)(a.Tq - end) * a.H * (D / 8);
-    uint4* z = (uint4*)((T*)a.out + (size_t)end * a.H * D);
+    const int start = min(max(a.cu_q[0], 0), a.Tq), end = min(max(a.cu_q[a.B], start), a.Tq);
+    const long long row = (long long)a.H * (D / 8), front = start * row, n = front + (a.Tq - end) * row;
+    uint4* z = (uint4*)a.out;
     for (long long i = (long long)blockIdx.x * 64 + tid - 320; i < n; i += (long long)gridDim.x * 64)
-      z[i] = make_uint4(0, 0, 0, 0);
+      z[i < front ? i : i - front + end * row] = make_uint4(0, 0, 0, 0);
   }
   tm_before();
   __syncthreads();

@@ -501,6 +501,37 @@ def test_prompt_attention_nonfinite_tokens(D, what):
             assert not got[at:200].isfinite().any()
 
 
+@gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_before_the_first_and_behind_the_last_sequence(D):
+    """Rows of no sequence are 0 wherever they lie."""
+    torch, _ = _torch()
+    randn = _gen(31)
+    q, k, v = randn(300, 4, D).half(), randn(300, 2, D).half(), randn(300, 2, D).half()
+    cu = torch.tensor([7, 200, 290], dtype=torch.int32, device="cuda")
+    got = mb.prompt_attention(q, k, v, cu)
+    assert (got[:7] == 0).all() and (got[290:] == 0).all()
+    for a, b in ((7, 200), (200, 290)):
+        ref, big = _attend(q[a:b], k[a:b], v[a:b], 0, D ** -0.5)
+        _close(got[a:b], ref, U["f16"] * ref.abs() + (U["f16"] + 2.0 ** -12) * big + 2.0 ** -20)
+    pool, table, kept = _kv4_case([90], 2, D, 32)
+    t = torch.tensor([90], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([3, 5], dtype=torch.int32, device="cuda")
+    got = mb.kv4_attention(q[:8], pool, table, t, cu)
+    assert (got[:3] == 0).all() and (got[5:] == 0).all()
+    ref, big = _attend(q[3:5], *kept[0], 88, D ** -0.5)
+    _close(got[3:5], ref, U["f16"] * ref.abs() + (2.0 ** -11 + 2.0 ** -12) * big + 90 * 2.0 ** -22)
+
+
+@gpu
+def test_paged_slots_past_31_bits():
+    """A page whose slots no int32 can name gives -1."""
+    torch, _ = _torch()
+    t = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    step = mb.paged_slots(t(0, 0), t(2, 2), t(-1, -1).view(2, 1), t(5, 2 ** 30), t(2), 4, 64)
+    assert step.slots.tolist() == [-1, -1, 320, 321]
+
+
 # ------------------------------------------------------------------ refusals
 P = 4096  # an address that no refused call reads
 
