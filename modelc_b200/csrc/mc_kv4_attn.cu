@@ -39,8 +39,12 @@ namespace mc {
 // rings share: 12 warps of 2 pages of D = 128 (4 of D = 64) for 8 query rows,
 // 8 warps of 3 (6) for 16 rows, whose accumulators take the registers.  (16
 // warps of 128 registers, two to a ring and each on half of every page, were
-// slower, 88 against 78 us for 273 MB: what bounds the kernel is the issue of
-// logic and f16 instructions, two cycles each, not their latency.)
+// slower, 88 against 78 us for 273 MB.)  What bounds a call of 74 us over
+// 273 MB: copies of the kernel without the f16 arithmetic, without the logic,
+// the tensor products, the scaling or the exponentials save 4 us at most each,
+// one that only loads takes 61, and one that loads no page still takes 24: the
+// start (a chain of loads of 1 us each to the first page, cold code) and the
+// join of the parts.
 template <int NP>
 constexpr int kKv4Warps = NP == 1 ? 12 : 8;
 constexpr int kKv4Rings = 24 * kv4_page_bytes(128);
@@ -537,9 +541,14 @@ __global__ void __launch_bounds__(32 * kKv4Warps<NP>, 1) k_kv4(const Kv4Args a) 
       if (!failed && s_there[wid][st]) {
         const uint8_t* pg = ring + st * PB;
         const int base = page * kKv4Page;
+        // Half pages, in a loop that stays one: with the whole page written out
+        // the code is longer, and it is fetched cold (one request of 1100
+        // tokens: 14.1 against 14.3 us; 770 MB of pages: 161.6 against 160.9).
+        // Pages that every row sees whole have a copy without masks all the
+        // same (188 us without it against 174, on a slower GPU).
         if (base + 64 <= first) {
-          step(pg, pg + 64 * D, base, std::false_type());
-          step(pg + 16 * D, pg + 66 * D, base + 32, std::false_type());
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) step(pg + h * 16 * D, pg + 64 * D + h * 2 * D, base + 32 * h, std::false_type());
         } else {
 #pragma unroll 1
           for (int h = 0; h < 2; ++h) step(pg + h * 16 * D, pg + 64 * D + h * 2 * D, base + 32 * h, std::true_type());
