@@ -17,14 +17,18 @@
 //   scores:  S^T = K Q^T with mma.m16n8k16, 16 tokens as rows, 8 query rows as
 //     columns; the block scale comes in in f32: S += (block's product) d.
 //   values:  O^T = V^T P^T, 16 dimensions as rows; p takes the block's scale
-//     with it, P' = f16(p d) <= 65504, and is transposed in registers.
+//     with it, P' = f16(p d), and is transposed in registers.
 // Feeding the bare codes as f16 subnormals (one AND) and taking -8 off by a
 // second product was built first: the tensor cores align subnormal factors
 // as if they were 2^-14, which left errors of 2^-13 of a block's scale.
-// Accumulation, softmax statistics and merging are f32.  P' in f16 (relative
-// 2^-11) and the query in f16, scaled by a power of two per row (exact for
-// bf16, and for f16 but for values 2^-24 below the row's largest), are the
-// only roundings besides the output's.
+// Accumulation, softmax statistics and merging are f32.  P' in f16 and the
+// query in f16, scaled by a power of two per row (exact for bf16, and for f16
+// but for values 2^-24 below the row's largest), are the only roundings besides
+// the output's.  The weights are p = 2^(score - reference + K), with K such
+// that p times the largest value scale so far stays below 2^14 (kv4_up): p d
+// keeps f16's 11 bits down to 2^-28 of the largest and 2^-25 absolute below, so
+// a row of small values, or one whose mass a single key takes, keeps its
+// small weights too.
 #include <math.h>
 
 #include <algorithm>
@@ -52,6 +56,18 @@ constexpr int kKv4Rings = 24 * kv4_page_bytes(128);
 // log2 units: weights are 2^(score - reference) <= 1, and the accumulators
 // are rescaled only when a score passes the reference.
 constexpr float kKv4Headroom = 2.f;
+// K for value scales below 2^(e - 14), e an f16 exponent field (0 for the
+// subnormal ones, 30 for the largest).  In bf16 calls p itself is rounded to
+// f16 before the product (short), and held below 2^14 where both factors then
+// have 22 bits of range at least (kv4_short: the largest scale between 2^-7 and
+// 2^6, values of 0.06 to 500).  Other calls round once, p d in f32 to f16: 770
+// MB take 178 us so, and 158 the short way.  Following the largest scale costs
+// 2 to 3 us of that.
+template <bool SHORT>
+__device__ __forceinline__ float kv4_up(int e) {
+  return (float)(SHORT && e >= 8 ? min(14, 28 - e) : 28 - e);
+}
+__device__ __forceinline__ bool kv4_short(int e) { return e >= 8 && e <= 20; }
 
 struct Kv4Args {
   const void* q;  // [T][H][D] with strides
@@ -127,6 +143,19 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // an 8x8 matrix o
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
+}
+
+// Two f16 without signs, as whole numbers: the larger ones (not NaN), and
+// whether one is at least its bound.
+__device__ __forceinline__ uint32_t max_pair(uint32_t x, uint32_t y) {
+  uint32_t z;
+  asm("max.f16x2 %0, %1, %2;" : "=r"(z) : "r"(x), "r"(y));
+  return z;
+}
+__device__ __forceinline__ bool reaches(uint32_t x, uint32_t bound) {
+  uint32_t z;
+  asm("set.ge.u32.f16x2 %0, %1, %2;" : "=r"(z) : "r"(x), "r"(bound));
+  return z != 0;
 }
 
 // The f16 pair (c - 8) of the codes in the low (ODD = 0) or second nibbles of
@@ -279,7 +308,8 @@ __global__ void __launch_bounds__(32 * kKv4Warps<NP>, 1) k_kv4(const Kv4Args a) 
   const int d_off = ((g & 1) * 4 + ((g >> 1) ^ ((g & 1) * 2))) * NB * 4;
   const int t_off[2] = {t * NB * 4, (4 + (t ^ 2)) * NB * 4};
   // For bf16 outputs p and its product with the scale are both rounded to f16:
-  // twice 2^-11 against the output's 2^-8 (a fifth fewer instructions).
+  // twice 2^-11 against the output's 2^-8 (a fifth fewer instructions).  Pages
+  // under a mask, and value scales that kv4_short excludes, have p d rounded once.
   constexpr bool FAST = std::is_same<T, __nv_bfloat16>::value;
 
   int st = 0, phase = 0;
@@ -338,6 +368,8 @@ __global__ void __launch_bounds__(32 * kKv4Warps<NP>, 1) k_kv4(const Kv4Args a) 
           bq[k * (D / 64) + w / 2][p][w & 1] = f2h(x[2 * k][w] * f, x[2 * k + 1][w] * f);
     }
     }
+    int big = 0;  // exponent field of the largest value scale so far
+    float up = kv4_up<FAST>(0);
     float o[NV][NP][4];
 #pragma unroll
     for (int x = 0; x < NV; ++x)
@@ -434,8 +466,8 @@ __global__ void __launch_bounds__(32 * kKv4Warps<NP>, 1) k_kv4(const Kv4Args a) 
       }
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
-        const float2 mc = make_float2(m[p].x == -INFINITY ? 0.f : -m[p].x * cs[p].x,
-                                      m[p].y == -INFINITY ? 0.f : -m[p].y * cs[p].y);
+        const float2 mc = make_float2(m[p].x == -INFINITY ? 0.f : fmaf(-m[p].x, cs[p].x, up),
+                                      m[p].y == -INFINITY ? 0.f : fmaf(-m[p].y, cs[p].y, up));
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -541,12 +573,46 @@ __global__ void __launch_bounds__(32 * kKv4Warps<NP>, 1) k_kv4(const Kv4Args a) 
       if (!failed && s_there[wid][st]) {
         const uint8_t* pg = ring + st * PB;
         const int base = page * kKv4Page;
+        // --- the page's value scales, one group and scale entry a lane: should
+        // one pass the largest so far, the weights come down
+        uint32_t vd[NB];
+        if constexpr (NB == 4) *(uint4*)vd = *(const uint4*)(pg + 68 * D + lane * 16);
+        else *(uint2*)vd = *(const uint2*)(pg + 68 * D + lane * 8);
+        uint32_t vt = vd[0] & 0x7fff7fffu;
+#pragma unroll
+        for (int b = 1; b < NB; ++b) vt = max_pair(vt, vd[b] & 0x7fff7fffu);
+        if (__any_sync(~0u, reaches(vt, (uint32_t)(big + 1) * 0x04000400u))) {
+          int e = 0;
+          const int kv = __ldg(a.kv_len + s_place[wid].z);
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              // scales that are not finite reach their sums as they are, and
+              // those behind the last token none
+              const int x = vd[b] >> (16 * h) & 0x7fff;
+              if (x < 0x7c00 && base + 8 * (lane >> 2) + kv4_token(2 * t + h) < kv) e = max(e, x >> 10);
+            }
+          e = __reduce_max_sync(~0u, e);
+          if (e > big) {
+            const float to = kv4_up<FAST>(e), f = ex2(to - up);
+            big = e, up = to;
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+              l[p].x *= f, l[p].y *= f;
+#pragma unroll
+              for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[v][p][c] *= f;
+            }
+          }
+        }
         // Half pages, in a loop that stays one: with the whole page written out
         // the code is longer, and it is fetched cold (one request of 1100
         // tokens: 14.1 against 14.3 us; 770 MB of pages: 161.6 against 160.9).
         // Pages that every row sees whole have a copy without masks all the
         // same (188 us without it against 174, on a slower GPU).
-        if (base + 64 <= first) {
+        if (base + 64 <= first && (!FAST || kv4_short(big))) {
 #pragma unroll 1
           for (int h = 0; h < 2; ++h) step(pg + h * 16 * D, pg + 64 * D + h * 2 * D, base + 32 * h, std::false_type());
         } else {
@@ -587,7 +653,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps<NP>, 1) k_kv4(const Kv4Args a) 
         const float sum = failed ? __int_as_float(0x7fffffff) : e ? l[p].y : l[p].x;
         if (!all && g == 0) {
           float* ml = a.ml + ((size_t)slot * R + row) * 2;
-          ml[0] = top == -INFINITY ? -INFINITY : top * (e ? cs[p].y : cs[p].x);
+          ml[0] = top == -INFINITY ? -INFINITY : fmaf(top, e ? cs[p].y : cs[p].x, -up);
           ml[1] = sum;
         }
         const float f = all ? (sum != 0.f ? 1.f / sum : 0.f) : 1.f;
