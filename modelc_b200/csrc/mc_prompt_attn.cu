@@ -16,7 +16,7 @@
 //     row, so maxima and sums need no exchange.
 // While one tile's rows are in the softmax the tensor cores work on the
 // other tile.  Scores, statistics and O are f32; P is rounded to the inputs'
-// type.  The reference of the exponentials follows the running maximum only
+// type (11 bits from f16, 8 from bf16).  The reference of the exponentials follows the running maximum only
 // when that has grown by more than 2^8: O is then rescaled in tensor memory.
 #include <cuda.h>
 #include <math.h>
@@ -37,6 +37,11 @@ constexpr int kPromptThreads = 384;
 // barrier is two phases ahead of a waiting load.
 constexpr int kPromptRounds = 8;
 constexpr float kPromptGrow = 8.f;  // log2 growth of the maximum that is let pass
+// Weights of f16 inputs are 2^7 larger, so that they reach 2^15 at most and keep
+// their 11 bits down to 2^-21 of the first reference: without it the small ones
+// of a row whose mass one key takes were subnormal.
+template <typename T>
+constexpr float kPromptUp = std::is_same<T, __half>::value ? 7.f : 0.f;
 
 struct PromptArgs {
   const void *q, *k, *v;  // [Tq][H][D], [Tk][Hk][D] with strides (elements)
@@ -476,7 +481,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
         m = mn;
       }
-      const float mc = m == -INFINITY ? 0.f : m * c;
+      const float mc = m == -INFINITY ? 0.f : fmaf(m, c, -kPromptUp<T>);
       float2 sum[2] = {};
       // (a cubic on the f32 pipes for a part of the exponentials was measured
       // slower, 936 against 977 TFLOP/s: the special function unit is not

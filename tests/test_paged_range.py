@@ -173,3 +173,21 @@ def test_kv4_attention_alone_and_among_others():
     ref, var = _exact(q[:20], kc, vc, torch.full((20,), n, device="cuda"), D ** -0.5)
     for got in (many[:20], alone):
         _within(got, ref, var, "bf16", 2.0 ** -11 * 2 ** 0.5)
+
+
+# ----------------------------------------------------------- packed prompts
+@gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("H,Hk,D", [(8, 2, 64), (8, 2, 128), (3, 3, 128)])
+@pytest.mark.parametrize("n,size,mass", [(4700, 1.0, 0.9), (4700, 1.0, 0.99), (4700, 0.01, 0.99), (20001, 1.0, 0.9),
+                                         (4700, 100.0, 0)])
+def test_prompt_attention_small_weights(dtype, H, Hk, D, n, size, mass):
+    """The last 300 tokens of a prompt behind a prefix."""
+    import torch
+    T = 300
+    q, k, v = (x.to(torch.float16 if dtype == "f16" else torch.bfloat16)
+               for x in _inputs(n, T, H, Hk, D, size, mass, n + D))
+    cu = lambda m: torch.tensor([0, m], dtype=torch.int32, device="cuda")  # noqa: E731
+    got = mb.prompt_attention(q, k, v, cu(T), cu(n))
+    ref, var = _exact(q, k, v, n - T + 1 + torch.arange(T, device="cuda"), D ** -0.5)
+    _within(got, ref, var, dtype, U[dtype])
