@@ -50,11 +50,15 @@ struct SlotArgs {
 // written into the table by the token that opens it (the one at a multiple
 // of the page size), so tables cost no loop of their own.  The scan reads
 // 8 B bytes from L2 in every block; what bounds the call is its latency.
+// Lengths may be any int32: sums are taken in 64 bits, a position that passes
+// 31 bits has no page, and what is written stops at kSlotMax.
 constexpr int kSlotThreads = 1024;
+constexpr int kSlotMax = 0x7fffffff;
 
 __global__ void __launch_bounds__(kSlotThreads) k_paged_slots(const SlotArgs a) {
-  __shared__ int s_cu[kSlotThreads], s_start[kSlotThreads], s_kv[kSlotThreads];
-  __shared__ int w_tok[32], w_pg[32];
+  __shared__ long long s_cu[kSlotThreads], s_start[kSlotThreads];
+  __shared__ int s_kv[kSlotThreads];
+  __shared__ long long w_tok[32], w_pg[32];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int per = (int)(((long long)a.tokens + gridDim.x - 1) / gridDim.x);
   const long long lo = (long long)blockIdx.x * per;
@@ -70,49 +74,50 @@ __global__ void __launch_bounds__(kSlotThreads) k_paged_slots(const SlotArgs a) 
       q = max(a.q_len[z], 0);
     }
     const int have = (int)min(((long long)kv + a.page - 1) / a.page, (long long)a.width);
-    const int need = (int)min(((long long)kv + q + a.page - 1) / a.page, (long long)a.width);
-    int tok = q, pg = need - have;  // inclusive sums over the chunk
+    const int all = (int)min((long long)kv + q, (long long)kSlotMax);
+    const int need = (int)min(((long long)all + a.page - 1) / a.page, (long long)a.width);
+    long long tok = q, pg = need - have;  // inclusive sums over the chunk
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(~0u, tok, o), y = __shfl_up_sync(~0u, pg, o);
+      const long long x = __shfl_up_sync(~0u, tok, o), y = __shfl_up_sync(~0u, pg, o);
       if (lane >= o) tok += x, pg += y;
     }
     if (lane == 31) w_tok[wid] = tok, w_pg[wid] = pg;
     __syncthreads();
     if (wid == 0) {
-      int x = w_tok[lane], y = w_pg[lane];
+      long long x = w_tok[lane], y = w_pg[lane];
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(~0u, x, o), v = __shfl_up_sync(~0u, y, o);
+        const long long u = __shfl_up_sync(~0u, x, o), v = __shfl_up_sync(~0u, y, o);
         if (lane >= o) x += u, y += v;
       }
       w_tok[lane] = x, w_pg[lane] = y;
     }
     __syncthreads();
     if (wid) tok += w_tok[wid - 1], pg += w_pg[wid - 1];
-    const int n_tok = w_tok[31], n_pg = w_pg[31];
+    const long long n_tok = w_tok[31], n_pg = w_pg[31];
     s_cu[tid] = tok - q;  // tokens of the chunk before this request
     s_start[tid] = pg - (need - have) - have;
     s_kv[tid] = kv;
     if (blockIdx.x == 0 && z < a.B) {
-      a.cu_q[z + 1] = (int)(base_tok + tok);
-      a.new_len[z] = kv + q;
+      a.cu_q[z + 1] = (int)min(base_tok + tok, (long long)kSlotMax);
+      a.new_len[z] = all;
     }
     __syncthreads();
     // this chunk's tokens are [base_tok, base_tok + n_tok)
     const long long t0 = max(lo, base_tok), t1 = min(hi, base_tok + n_tok);
     const int nz = min(kSlotThreads, a.B - z0);
     for (long long t = t0 + tid; t < t1; t += kSlotThreads) {
-      const int i = (int)(t - base_tok);
+      const long long i = t - base_tok;
       int l = 0, r = nz;  // the last request that starts at or before token i
       while (r - l > 1) {
         const int m = (l + r) >> 1;
         if (s_cu[m] <= i) l = m;
         else r = m;
       }
-      const int kvl = s_kv[l], pos = kvl + i - s_cu[l], j = pos / a.page;
+      const int kvl = s_kv[l], pos = (int)min(kvl + (i - s_cu[l]), (long long)kSlotMax), j = pos / a.page;
       int page = -1;
-      if (j < a.width) {
+      if (j < a.width && pos < kSlotMax) {
         int* entry = a.table + (size_t)(z0 + l) * a.width + j;
         if ((long long)j * a.page >= kvl) {
           const long long nth = (long long)n_free - 1 - (base_pg + s_start[l] + j);
@@ -134,7 +139,7 @@ __global__ void __launch_bounds__(kSlotThreads) k_paged_slots(const SlotArgs a) 
     a.positions[t] = 0;
     a.slots[t] = -1;
   }
-  if (blockIdx.x == 0 && tid == 0) *a.n_free_out = (int)(*a.n_free - base_pg);
+  if (blockIdx.x == 0 && tid == 0) *a.n_free_out = (int)max(*a.n_free - base_pg, -(long long)kSlotMax);
 }
 
 // -------------------------------------------------------- rotary positions
