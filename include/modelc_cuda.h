@@ -444,9 +444,12 @@ MC_API mc_status mc_sample_rows(const float* logits_dev, int32_t n_rows, int32_t
  * position 0 and slot -1; new_len = kv_len + q_len; *n_free_out = *n_free
  * minus the pages taken.  When the stack runs out *n_free_out is negative
  * (the pages missing) and the tokens without a page get table entry and slot
- * -1, as tokens beyond table_width pages get slot -1.  n_tokens must be at
- * least the sum of q_len: tokens beyond it are not placed.  Inputs other than
- * the table are left as they are, so a step can be planned again. */
+ * -1, as tokens beyond table_width pages get slot -1.  n_tokens should be at
+ * least the sum of q_len: tokens beyond it get no position and no slot, though
+ * their pages are taken and entered.  Lengths may be any int32: a position
+ * past 31 bits has no page, and cu_q, positions and new_len stop at 2^31 - 1.
+ * Inputs other than the table are left as they are, so a step can be planned
+ * again. */
 typedef struct mc_slots_args {
   const int32_t *kv_len, *q_len;
   int32_t* table;

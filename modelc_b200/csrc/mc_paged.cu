@@ -131,6 +131,15 @@ __global__ void __launch_bounds__(kSlotThreads) k_paged_slots(const SlotArgs a) 
       const long long slot = (long long)page * a.page + pos % a.page;
       a.slots[t] = page < 0 || slot > 0x7fffffffll ? -1 : (int)slot;
     }
+    // requests that the output cuts off: the pages that the tokens behind its
+    // end open are taken all the same, so they have to be in the table
+    if (base_tok + tok > a.tokens) {
+      const long long placed = max(a.tokens - (base_tok + tok - q), 0ll);
+      for (long long j = (kv + placed + a.page - 1) / a.page + blockIdx.x; j < need; j += gridDim.x) {
+        const long long nth = (long long)n_free - 1 - (base_pg + s_start[tid] + j);
+        a.table[(size_t)z * a.width + j] = nth >= 0 && nth < a.n_pages_free ? a.free_pages[nth] : -1;
+      }
+    }
     base_tok += n_tok;
     base_pg += n_pg;
     __syncthreads();

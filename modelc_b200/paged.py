@@ -97,7 +97,8 @@ def paged_slots(kv_len, q_len, table, free_pages, n_free, tokens: int, page_size
     """Plans a step: request z holds kv_len[z] tokens and gets q_len[z] new
     ones; missing pages come from the top of the stack free_pages[:n_free]
     and are entered into table [requests, width] in place.  ``tokens`` is the
-    output's length, at least the sum of q_len (mc_paged_slots)."""
+    output's length, at least the sum of q_len: tokens behind it get no slot,
+    but their pages are taken and entered (mc_paged_slots)."""
     dev = _gpu(kv_len, "kv_len")
     n = kv_len.shape[0]
     if table.dim() != 2 or table.shape[0] != n:
