@@ -423,8 +423,8 @@ MC_API mc_status mc_sample_rows(const float* logits_dev, int32_t n_rows, int32_t
  * whose caches are f32 or int8 and live on the host.
  *
  * Every pointer is device memory of `device`, every call is asynchronous on
- * `stream` (a cudaStream_t as void*), allocates nothing and can be captured
- * in a CUDA graph.  Index arrays are int32.  Strides count elements; the last
+ * `stream` (a cudaStream_t as void*), allocates nothing, leaves the caller's
+ * current device as it was and can be captured in a CUDA graph.  Index arrays are int32.  Strides count elements; the last
  * axis of an activation is contiguous.  Sizes of zero are valid and do
  * nothing.
  */

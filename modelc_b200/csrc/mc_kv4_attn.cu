@@ -855,7 +855,7 @@ using namespace mc;
 
 extern "C" int64_t mc_kv4_attention_workspace(int32_t n_requests, int32_t head_dim, int32_t device) {
   if (n_requests < 0 || (head_dim != 64 && head_dim != 128)) return 0;
-  if (paged_device(device) != MC_OK) return 0;
+  if (paged_check(device) != MC_OK) return 0;
   const int sms = paged_sms(device);
   return (int64_t)std::max(kv4_space(sms, n_requests, 8, head_dim).total,
                            kv4_space(sms, n_requests, 16, head_dim).total);
@@ -888,7 +888,7 @@ extern "C" mc_status mc_kv4_attention(const mc_kv4_attention_args* args, int32_t
     return set_error(MC_E_INVALID, "null pointer");
   if ((n_pages && !aligned(pool, 16)) || !aligned(workspace, 16))
     return set_error(MC_E_INVALID, "pool and workspace must be 16-byte aligned");
-  MC_PCKS(paged_device(device));
+  MC_PAGED_DEVICE(device);
   const int sms = paged_sms(device), rows = kv4_rows(n_tokens, n_requests, n_heads, n_kv_heads);
   const Kv4Space sp = kv4_space(sms, n_requests, rows, head_dim);
   if (workspace_bytes < (int64_t)sp.total) return set_error(MC_E_CAPACITY, "workspace too small");

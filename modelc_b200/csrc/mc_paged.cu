@@ -11,7 +11,7 @@ namespace mc {
 constexpr int kMaxDevices = 64;
 static std::atomic<int> g_sms[kMaxDevices];  // SM count once checked, 0 before
 
-mc_status paged_device(int device) {
+mc_status paged_check(int device) {
   if (device < 0 || device >= kMaxDevices) return set_error(MC_E_INVALID, "bad device index");
   if (!g_sms[device].load(std::memory_order_acquire)) {
     int n = 0;
@@ -27,10 +27,18 @@ mc_status paged_device(int device) {
     if (major != 10 || minor != 0) return set_error(MC_E_CUDA, "not an sm_100 device");
     g_sms[device].store(sms, std::memory_order_release);
   }
-  int cur = -1;
-  MC_PCK(cudaGetDevice(&cur));
-  if (cur != device) MC_PCK(cudaSetDevice(device));
   return MC_OK;
+}
+
+PagedDevice::PagedDevice(int device) : status(paged_check(device)) {
+  if (status != MC_OK) return;
+  int cur = -1;
+  cudaError_t e = cudaGetDevice(&cur);
+  if (e == cudaSuccess && cur != device) {
+    e = cudaSetDevice(device);
+    back_ = cur;
+  }
+  if (e != cudaSuccess) status = set_error(MC_E_CUDA, cudaGetErrorString(e));
 }
 
 int paged_sms(int device) { return g_sms[device].load(std::memory_order_acquire); }
@@ -516,7 +524,7 @@ extern "C" mc_status mc_paged_slots(const mc_slots_args* args, int32_t device, v
       (n_requests > 0 && table_width > 0 && !table) || (n_free_pages > 0 && !free_pages) ||
       (n_tokens > 0 && (!positions || !slots)))
     return set_error(MC_E_INVALID, "null pointer");
-  MC_PCKS(paged_device(device));
+  MC_PAGED_DEVICE(device);
   SlotArgs a{kv_len, q_len, table, free_pages, n_free, cu_q, positions, slots, new_len, n_free_out,
              n_requests, table_width, page_size, n_tokens, n_free_pages};
   const int grid = std::max(1, std::min(paged_sms(device), n_tokens / kSlotThreads + 1));
@@ -530,7 +538,7 @@ extern "C" mc_status mc_rope_table(const double* freq, int32_t n_freq, int32_t p
                                    void* stream) {
   if (n_freq <= 0 || positions <= 0) return set_error(MC_E_SHAPE, "empty table");
   if (!freq || !cos_out || !sin_out) return set_error(MC_E_INVALID, "null pointer");
-  MC_PCKS(paged_device(device));
+  MC_PAGED_DEVICE(device);
   const long long n = (long long)positions * n_freq;
   const int grid = (int)std::min<long long>((n + 255) / 256, 8ll * paged_sms(device));
   k_rope_table<<<grid, 256, 0, (cudaStream_t)stream>>>(freq, n_freq, positions, factor, cos_out, sin_out);
@@ -563,7 +571,7 @@ extern "C" mc_status mc_rope(const mc_rope_args* args, int32_t device, void* str
     return set_error(MC_E_INVALID, "null pointer");
   if ((long long)n_tokens * (n_heads + n_kv_heads) * (head_dim / 2) >= (1ll << 31) * 4)
     return set_error(MC_E_CAPACITY, "too many values for one call");
-  MC_PCKS(paged_device(device));
+  MC_PAGED_DEVICE(device);
   RopeArgs a{q, k, q_out, k_out, q_tok, q_head, k_tok, k_head, positions, cos_table, sin_table,
              n_tokens, n_heads, n_kv_heads, head_dim, rot, table_rows, 0};
   // Groups of four values where all sizes, strides and addresses allow the
@@ -621,7 +629,7 @@ extern "C" mc_status mc_kv4_append(const mc_kv4_append_args* args, int32_t devic
   if (!k || !v || !slots) return set_error(MC_E_INVALID, "null pointer");
   if ((long long)n_tokens * n_kv_heads > 0x7fffffffll)
     return set_error(MC_E_CAPACITY, "too many rows for one call");
-  MC_PCKS(paged_device(device));
+  MC_PAGED_DEVICE(device);
   AppendArgs a{k, v, k_tok, k_head, v_tok, v_head, slots, (uint8_t*)pool, n_tokens, n_kv_heads,
                (int)(n_pages * kKv4Page)};
   MC_PCK(head_dim == 128 ? (by_type<Append, 128>(dtype, a, device, (cudaStream_t)stream))
@@ -646,7 +654,7 @@ extern "C" mc_status mc_kv4_read(const mc_kv4_read_args* args, int32_t device, v
     return set_error(MC_E_INVALID, "outputs must be 16-byte aligned");
   if ((long long)n_tokens * n_kv_heads > 0x7fffffffll)
     return set_error(MC_E_CAPACITY, "too many rows for one call");
-  MC_PCKS(paged_device(device));
+  MC_PAGED_DEVICE(device);
   ReadArgs a{(const uint8_t*)pool, slots, k_out, v_out, n_tokens, n_kv_heads, (int)(n_pages * kKv4Page)};
   MC_PCK(head_dim == 128 ? (by_type<Read, 128>(dtype, a, device, (cudaStream_t)stream))
                          : (by_type<Read, 64>(dtype, a, device, (cudaStream_t)stream)));

@@ -14,9 +14,25 @@ namespace mc {
 
 mc_status set_error(mc_status st, const char* msg);  // mc_api.cu
 
-// Makes `device` current after checking once that it is an sm_100 device.
-mc_status paged_device(int device);
-int paged_sms(int device);  // its SM count (after paged_device)
+// Checks, once a device, that it is an sm_100 device.
+mc_status paged_check(int device);
+int paged_sms(int device);  // its SM count (after paged_check)
+
+// Makes a checked device current, and the caller's current again at the end of
+// the scope; does nothing where they are the same.
+class PagedDevice {
+ public:
+  explicit PagedDevice(int device);
+  ~PagedDevice() {
+    if (back_ >= 0) cudaSetDevice(back_);
+  }
+  PagedDevice(const PagedDevice&) = delete;
+  PagedDevice& operator=(const PagedDevice&) = delete;
+  mc_status status;
+
+ private:
+  int back_ = -1;
+};
 
 #define MC_PCK(call)                                                          \
   do {                                                                        \
@@ -25,6 +41,10 @@ int paged_sms(int device);  // its SM count (after paged_device)
       return ::mc::set_error(e_ == cudaErrorMemoryAllocation ? MC_E_OOM : MC_E_CUDA, \
                              cudaGetErrorString(e_));                         \
   } while (0)
+// For the rest of the function, or until it returns with the error.
+#define MC_PAGED_DEVICE(device)         \
+  ::mc::PagedDevice device_scope(device); \
+  if (device_scope.status != MC_OK) return device_scope.status
 #define MC_PCKS(expr)             \
   do {                            \
     mc_status s_ = (expr);        \

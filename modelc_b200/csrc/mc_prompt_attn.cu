@@ -640,7 +640,7 @@ extern "C" mc_status mc_prompt_attention(const mc_prompt_args* args, int32_t dev
   const long long blocks = (((long long)n_q + rows - 1) / rows + n_sequences) * units;
   if (blocks > 0x7fffffffll || n_q > 0x7fffff00 || n_k > 0x7fffff00)
     return set_error(MC_E_CAPACITY, "too many rows for one call");
-  MC_PCKS(paged_device(device));
+  MC_PAGED_DEVICE(device);
   cudaStream_t s = (cudaStream_t)stream;
   if (n_k == 0 || n_sequences == 0) {  // no row sees a key
     MC_PCK(cudaMemsetAsync(out, 0, (size_t)n_q * n_heads * head_dim * 2, s));
