@@ -5,7 +5,9 @@ Each function checks its tensors, allocates its outputs with torch and makes
 one asynchronous call of the C ABI (include/modelc_cuda.h) on the current
 stream of the tensors' device; the arithmetic is described there.  Tensors
 used on another stream than the one they were allocated on need torch's usual
-care (record_stream or events).
+care (record_stream or events).  The operators have no backward pass: results
+of inputs that want gradients raise when these are asked for, and what
+kv4_append stores carries none.
 
 Decode steps make these calls with a few tokens each, where the host's time is
 the whole cost: the argument structs are packed with ``struct`` and passed as
@@ -82,6 +84,20 @@ def _gpu(t: torch.Tensor, name: str) -> int:
 
 def _like(t: torch.Tensor, dtype=None) -> torch.Tensor:
     return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
+
+
+class _NoBackward(torch.autograd.Function):
+    """Keeps a result in the graph of inputs that want gradients, so that asking
+    for them is an error and not a silent zero."""
+
+    @staticmethod
+    def forward(ctx, name, out, *inputs):
+        ctx.name = name
+        return out
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise NotImplementedError(f"{ctx.name} has no backward pass")
 
 
 class PagedStep(NamedTuple):
@@ -214,6 +230,9 @@ def rope(q, k, positions, cos, sin, layout: str = "half", dtype=None):
     check(lib().mc_rope(_ROPE(q.data_ptr(), kp, pos, cos.data_ptr(), sin.data_ptr(), qo.data_ptr(), kop, q0, q1,
                               k0, k1, H, Hk, _ACT[own], _ACT[dtype], T, D, 2 * half, layout == "interleaved",
                               rows), dev, _stream(dev)))
+    if (q.requires_grad or k is not None and k.requires_grad) and torch.is_grad_enabled():
+        qo = _NoBackward.apply("rope", qo, q, k)
+        ko = None if ko is None else _NoBackward.apply("rope", ko, q, k)
     return qo, ko
 
 
@@ -302,6 +321,8 @@ def kv4_attention(q, pool, table, kv_len, cu_q, scale: float | None = None):
         q.data_ptr(), pool.data_ptr(), _index(table, "table", dev), _index(kv_len, "kv_len", dev),
         _index(cu_q, "cu_q", dev, (B + 1,)), out.data_ptr(), ws.data_ptr(), q0, q1, pages, n, _ACT[dt], T, H, Hk,
         D, table.shape[1], B, D ** -0.5 if scale is None else scale), dev, _stream(dev)))
+    if q.requires_grad and torch.is_grad_enabled():
+        out = _NoBackward.apply("kv4_attention", out, q)
     return out
 
 
@@ -330,4 +351,6 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, scale: float | None = None, causa
         q.data_ptr(), k.data_ptr(), v.data_ptr(), _index(cu_q, "cu_q", dev), _index(cu_k, "cu_k", dev, (B + 1,)),
         out.data_ptr(), q0, q1, k0, k1, v0, v1, _ACT[dt], T, Tk, H, Hk, D, B, causal,
         D ** -0.5 if scale is None else scale), dev, _stream(dev)))
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        out = _NoBackward.apply("prompt_attention", out, q, k, v)
     return out

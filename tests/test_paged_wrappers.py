@@ -1,0 +1,46 @@
+"""What the paged operators' torch functions do beside the kernels."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+import modelc_b200 as mb
+
+gpu = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@gpu
+@pytest.mark.parametrize("wants", ["q", "k", "v"])
+def test_gradients_are_refused_aloud(wants):
+    """A result of inputs that want gradients says so when they are asked for;
+    values and calls that want none are as ever."""
+    import torch
+    t = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    x = {n: torch.randn(5, 2, 64, generator=g, device="cuda").half() for n in "qkv"}
+    cos, sin = mb.rope_table(8, 64)
+    pool = mb.kv4_pool(1, 2, 64)
+    mb.kv4_append(pool, x["k"], x["v"], t(0, 1, 2, 3, 4))
+
+    def calls():
+        rope = mb.rope(x["q"], x["k"], t(0, 1, 2, 3, 4), cos, sin)
+        return {"rope": rope[0], "rope of k": rope[1], "rope of q": mb.rope(x["q"], None, t(*[0] * 5), cos, sin)[0],
+                "prompt_attention": mb.prompt_attention(x["q"], x["k"], x["v"], t(0, 5)),
+                "kv4_attention": mb.kv4_attention(x["q"], pool, t(0).view(1, 1), t(5), t(0, 5))}
+
+    plain = calls()
+    assert not any(y.requires_grad for y in plain.values())
+    x[wants].requires_grad_()
+    mb.kv4_append(pool, x["k"], x["v"], t(0, 1, 2, 3, 4))
+    reached = {"q": list(plain), "k": ["rope", "rope of k", "prompt_attention"], "v": ["prompt_attention"]}[wants]
+    for name, y in calls().items():
+        assert torch.equal(y.detach(), plain[name]) and y.requires_grad == (name in reached)
+        if name in reached:
+            with pytest.raises(NotImplementedError, match=name.split()[0]):
+                y.float().sum().backward()
+    with torch.no_grad():
+        assert not any(y.requires_grad for y in calls().values())
+    assert x[wants].grad is None
