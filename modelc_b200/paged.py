@@ -161,8 +161,12 @@ def rope_frequencies(rot: int, theta: float = 10000.0, scaling: RopeScaling | No
         raise ValueError("rot must be even and positive")
     if s.kind not in ("none", "linear", "ntk", "llama3", "yarn"):
         raise ValueError(f"unknown scaling {s.kind!r}")
-    if theta <= 0 or s.factor <= 0 or s.old_context <= 0:
+    if not all(0 < x < math.inf for x in (theta, s.factor, s.old_context)):
         raise ValueError("theta, factor and old_context must be positive")
+    if s.kind == "llama3" and not s.low_turns < s.high_turns:
+        raise ValueError("low_turns must be below high_turns")
+    if s.kind == "yarn" and not (theta > 1 and 0 < s.slow <= s.fast):
+        raise ValueError("yarn: theta above 1 and 0 < slow <= fast are wanted")
     if s.kind == "ntk":
         theta = theta * s.factor ** (rot / max(rot - 2, 1))
     f = [theta ** (-2.0 * i / rot) for i in range(rot // 2)]

@@ -44,3 +44,21 @@ def test_gradients_are_refused_aloud(wants):
     with torch.no_grad():
         assert not any(y.requires_grad for y in calls().values())
     assert x[wants].grad is None
+
+
+@pytest.mark.parametrize("theta,scaling", [
+    (1e4, dict(kind="llama3", low_turns=4.0, high_turns=4.0)), (1e4, dict(kind="llama3", low_turns=5.0)),
+    (1.0, dict(kind="yarn", factor=4.0)), (0.5, dict(kind="yarn", factor=4.0)),
+    (1e4, dict(kind="yarn", factor=4.0, slow=0.0)), (1e4, dict(kind="yarn", factor=4.0, fast=-1.0)),
+    (1e4, dict(kind="yarn", factor=4.0, slow=8.0, fast=2.0)), (1e4, dict(kind="linear", factor=float("nan"))),
+    (float("nan"), dict(kind="none")), (float("inf"), dict(kind="none"))], ids=str)
+def test_scalings_without_a_meaning_are_refused(theta, scaling):
+    with pytest.raises(ValueError, match="must be|wanted"):
+        mb.rope_frequencies(64, theta, mb.RopeScaling(**scaling))
+
+
+def test_scalings_at_the_edge_of_their_meaning():
+    assert mb.rope_frequencies(64, 1.0)[0] == [1.0] * 32
+    f, _ = mb.rope_frequencies(64, 1e4, mb.RopeScaling("llama3", 8.0, low_turns=3.999, high_turns=4.0))
+    assert all(a > b for a, b in zip(f, f[1:]))
+    mb.rope_frequencies(64, 1e4, mb.RopeScaling("yarn", 4.0, slow=2.0, fast=2.0))
