@@ -19,8 +19,9 @@ _PAGED = ("PagedStep", "RopeScaling", "kv4_append", "kv4_attention", "kv4_pool",
 
 
 def __getattr__(name):
-    if name in _PAGED:
-        from . import paged
+    if name == "paged" or name in _PAGED:
+        from importlib import import_module
+        paged = import_module(".paged", __name__)
         globals().update({n: getattr(paged, n) for n in _PAGED})
         return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -62,3 +62,12 @@ def test_scalings_at_the_edge_of_their_meaning():
     f, _ = mb.rope_frequencies(64, 1e4, mb.RopeScaling("llama3", 8.0, low_turns=3.999, high_turns=4.0))
     assert all(a > b for a, b in zip(f, f[1:]))
     mb.rope_frequencies(64, 1e4, mb.RopeScaling("yarn", 4.0, slow=2.0, fast=2.0))
+
+
+@pytest.mark.parametrize("use", ["mb.paged.PAGE == 64", "mb.rope_frequencies(8)[1] == 1.0",
+                                 "mb.paged.rope is mb.rope", "not hasattr(mb, 'paged_attention')"])
+def test_names_before_the_first_use(use):
+    """Everything is there in a fresh interpreter, whichever is asked for first."""
+    r = subprocess.run([sys.executable, "-c", f"import modelc_b200 as mb; assert {use}"], cwd=ROOT,
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-1000:]
