@@ -203,9 +203,28 @@ __device__ __forceinline__ void prompt_work(const PromptArgs& a, int index, Prom
   __syncwarp();
 }
 
+// The last key in [from, to) of the sequence at k0 whose V row holds a NaN or an
+// infinity, or -1.  A row whose result is not finite has it from the keys that
+// it sees, and then it is right, or from one of these behind them: the product
+// of a hidden key's weight 0 with its NaN or infinity is not 0.
+template <typename T, int D>
+__device__ __noinline__ int prompt_last_bad(const PromptArgs& a, int h, int k0, int from, int to) {
+  constexpr uint32_t kTop = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;  // exponents of those
+  const int lane = threadIdx.x & 31, x = lane % (D / 8);
+  const T* vp = (const T*)a.v + h / (a.H / a.Hk) * a.v_head + x * 8;
+  int last = -1;
+#pragma unroll 4
+  for (int j = from + lane / (D / 8); j < to; j += 256 / D) {
+    const uint4 y = *(const uint4*)(vp + (long long)(k0 + j) * a.v_tok);
+    const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+    for (int i = 0; i < 4; ++i)
+      if ((w[i] & kTop) == kTop || (w[i] >> 16 & kTop) == kTop) last = j;
+  }
+  return __reduce_max_sync(~0u, last);
+}
+
 // One row again, with a lane per key and then per column, over its own keys
-// alone: for rows whose result is not finite, since a product of a hidden
-// key's weight 0 with its NaN or infinity is not 0.
+// alone: for rows that a hidden key spoiled.
 template <typename T, int D>
 __device__ __noinline__ void prompt_row(const PromptArgs& a, int t, int h, int k0, int n) {
   constexpr int NB = D / 32;
@@ -221,7 +240,13 @@ __device__ __noinline__ void prompt_row(const PromptArgs& a, int t, int h, int k
     if (j < n) {
       const T* k = kp + (long long)(k0 + j) * a.k_tok;
       x = 0.f;
-      for (int i = 0; i < D; ++i) x += to_f(k[i]) * to_f(q[i]);
+#pragma unroll 4
+      for (int i = 0; i < D; i += 8) {
+        const uint4 kk = *(const uint4*)(k + i), qq = *(const uint4*)(q + i);
+        const T *ke = (const T*)&kk, *qe = (const T*)&qq;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x += to_f(ke[e]) * to_f(qe[e]);
+      }
       x *= a.scale;
     }
     float top = x;
@@ -232,11 +257,16 @@ __device__ __noinline__ void prompt_row(const PromptArgs& a, int t, int h, int k
     m = mn;
     l = l * c + e;
     for (int b = 0; b < NB; ++b) o[b] *= c;
+#pragma unroll 4
     for (int i = 0; i < min(32, n - j0); ++i) {
       const float p = __shfl_sync(~0u, e, i);
       const T* v = vp + (long long)(k0 + j0 + i) * a.v_tok;
       for (int b = 0; b < NB; ++b) o[b] += p * to_f(v[b * 32 + lane]);
     }
+    // nothing that follows changes a row that is NaN in every column
+    bool settled = true;
+    for (int b = 0; b < NB; ++b) settled = settled && o[b] != o[b];
+    if (__all_sync(~0u, settled)) break;
   }
   for (int f = 16; f; f >>= 1) l += __shfl_xor_sync(~0u, l, f);
   T* out = (T*)a.out + ((size_t)t * a.H + h) * D;
@@ -546,7 +576,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       for (int x = 0; x < D / 8; ++x) *(uint4*)(out + x * 8) = make_uint4(y, y, y, y);
     }
     __syncwarp();
-    for (unsigned again = __ballot_sync(~0u, bad && live); again; again &= again - 1) {
+    unsigned again = __ballot_sync(~0u, bad && live);
+    if (again) {
+      // the products reached whole groups of 16 keys; `see` grows along the rows
+      const int last = prompt_last_bad<T, D>(a, head_t, w.k0, __shfl_sync(~0u, see, __ffs(again) - 1),
+                                             min((lim[t] + 15) / 16 * 16, w.L));
+      again &= __ballot_sync(~0u, last >= see);
+    }
+    for (; again; again &= again - 1) {
       const int r = __ffs(again) - 1;
       prompt_row<T, D>(a, w.q0 + first + r, head_t, w.k0, __shfl_sync(~0u, see, r));
     }
