@@ -58,6 +58,12 @@ def _index(t: torch.Tensor, name: str, dev: int, shape=None) -> int:
     return t.data_ptr()
 
 
+def _length(t: torch.Tensor, name: str) -> int:
+    if t.dim() != 1:
+        raise ValueError(f"{name}: one axis is wanted")
+    return t.shape[0]
+
+
 def _heads(t: torch.Tensor, name: str, dev: int) -> torch.Tensor:
     """[tokens, heads, head_dim] on device `dev` with a contiguous last axis."""
     if t.dim() != 3 or t.get_device() != dev or t.dtype not in _ACT:
@@ -116,7 +122,7 @@ def paged_slots(kv_len, q_len, table, free_pages, n_free, tokens: int, page_size
     output's length, at least the sum of q_len: tokens behind it get no slot,
     but their pages are taken and entered (mc_paged_slots)."""
     dev = _gpu(kv_len, "kv_len")
-    n = kv_len.shape[0]
+    n = _length(kv_len, "kv_len")
     if table.dim() != 2 or table.shape[0] != n:
         raise ValueError(f"table: [{n}, width] is wanted")
     if tokens < 0:
@@ -124,6 +130,7 @@ def paged_slots(kv_len, q_len, table, free_pages, n_free, tokens: int, page_size
     kv = _index(kv_len, "kv_len", dev)
     q = _index(q_len, "q_len", dev, kv_len.shape)
     tab = _index(table, "table", dev)
+    n_pages = _length(free_pages, "free_pages")
     free = _index(free_pages, "free_pages", dev)
     left = _index(n_free, "n_free", dev, (1,))
     out = torch.empty(2 * (tokens + n + 1), dtype=_INT, device=kv_len.device)
@@ -131,7 +138,7 @@ def paged_slots(kv_len, q_len, table, free_pages, n_free, tokens: int, page_size
     pos = p + 4 * (n + 1)
     new = pos + 8 * tokens
     check(lib().mc_paged_slots(_SLOTS(kv, q, tab, free, left, p, pos, pos + 4 * tokens, new, new + 4 * n, n,
-                                      table.shape[1], free_pages.shape[0], page_size, tokens), dev, _stream(dev)))
+                                      table.shape[1], n_pages, page_size, tokens), dev, _stream(dev)))
     return PagedStep(*out.unsafe_split_with_sizes((n + 1, tokens, tokens, n, 1)))
 
 
@@ -262,7 +269,7 @@ def _pool(pool: torch.Tensor, head_dim: int) -> int:
 def kv4_append(pool, k, v, slots) -> None:
     """Quantizes k, v [tokens, kv heads, head_dim] into their slots of the
     pool (q4_0 blocks of 32 values); slots outside the pool are skipped."""
-    dev = _pool(pool, k.shape[-1])
+    dev = _pool(pool, k.shape[-1] if k.dim() else 0)
     k, v = _heads(k, "k", dev), _heads(v, "v", dev)
     T, Hk, D = k.shape
     if v.shape != k.shape or v.dtype is not k.dtype or Hk != pool.shape[1]:
@@ -310,7 +317,7 @@ def kv4_attention(q, pool, table, kv_len, cu_q, scale: float | None = None):
     dt = q.dtype
     if dt is not _BF16 and dt is not _F16:
         raise ValueError("q: f16 or bf16 is wanted")
-    B = kv_len.shape[0]
+    B = _length(kv_len, "kv_len")
     if table.dim() != 2 or table.shape[0] != B:
         raise ValueError(f"table: [{B}, width] is wanted")
     pages, Hk, _ = pool.shape
@@ -347,7 +354,7 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, scale: float | None = None, causa
         raise ValueError("k, v: one shape, with q's head dim, is wanted")
     (q, q0, q1), (k, k0, k1), (v, v0, v1) = _rows16(q), _rows16(k), _rows16(v)
     cu_k = cu_q if cu_k is None else cu_k
-    B = cu_q.shape[0] - 1
+    B = _length(cu_q, "cu_q") - 1
     if B < 0:
         raise ValueError("cu_q: [sequences + 1] is wanted")
     out = _like(q)

@@ -71,3 +71,21 @@ def test_names_before_the_first_use(use):
     r = subprocess.run([sys.executable, "-c", f"import modelc_b200 as mb; assert {use}"], cwd=ROOT,
                        capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-1000:]
+
+
+@gpu
+def test_lengths_of_one_axis_are_wanted():
+    """More axes were read as if the first ran through them, none gave an IndexError."""
+    import torch
+    i = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    x = torch.zeros(4, 2, 64, device="cuda", dtype=torch.float16)
+    pool = mb.kv4_pool(3, 2, 64)
+    for bad in (lambda: mb.paged_slots(i(2, 2), i(2, 2), i(2, 4), i(1), i(1), 4),
+                lambda: mb.paged_slots(i(), i(), i(1, 4), i(1), i(1), 4),
+                lambda: mb.paged_slots(i(2), i(2), i(2, 4), i(1, 3), i(1), 4),
+                lambda: mb.kv4_attention(x, pool, i(2, 3), i(2, 2), i(3)),
+                lambda: mb.kv4_attention(x, pool, i(1, 3), i(), i(2)),
+                lambda: mb.prompt_attention(x, x, x, i(2, 2)), lambda: mb.prompt_attention(x, x, x, i()),
+                lambda: mb.kv4_append(pool, x[0, 0, 0], x, i(4))):
+        with pytest.raises(ValueError):
+            bad()
