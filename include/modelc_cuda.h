@@ -517,7 +517,10 @@ MC_API mc_status mc_kv4_read(const mc_kv4_read_args* args, int32_t device, void*
  * the last of its kv_len[z] tokens (the cache holds them already): row j sees
  * the tokens up to its own.  A row that sees none, and a row of no request,
  * gives 0; a page whose table entry lies outside the pool counts as not
- * there.  q and out are f16 or bf16; out is contiguous.  The workspace
+ * there.  q and out are f16 or bf16; out is contiguous.  Scores, maxima and
+ * sums are f32; the weight of a token times its value scale is rounded to f16
+ * (in bf16 calls the weight before that too), kept in range by the largest
+ * scale of the visible tokens.  The workspace
  * (16-byte aligned, of the size that mc_kv4_attention_workspace gives, 0 on
  * an error) needs no clearing and is free again when the call has run. */
 typedef struct mc_kv4_attention_args {
@@ -537,7 +540,9 @@ MC_API mc_status mc_kv4_attention(const mc_kv4_attention_args* args, int32_t dev
  * at a multiple of 16 bytes).  Causal: the sequence's queries are its last
  * tokens, so query i sees the keys up to i + (keys - queries).  A row that
  * sees no key, and a row of no sequence, gives 0.  out is contiguous, of q's
- * type. */
+ * type.  Scores, maxima and sums are f32; weights are rounded to q's type for
+ * their product with v.  A NaN or an infinity reaches the rows that see it and
+ * no other. */
 typedef struct mc_prompt_args {
   const void *q, *k, *v;
   const int32_t *cu_q, *cu_k;

@@ -43,12 +43,12 @@ namespace mc {
 // rings share: 12 warps of 2 pages of D = 128 (4 of D = 64) for 8 query rows,
 // 8 warps of 3 (6) for 16 rows, whose accumulators take the registers.  (16
 // warps of 128 registers, two to a ring and each on half of every page, were
-// slower, 88 against 78 us for 273 MB.)  What bounds a call of 74 us over
-// 273 MB: copies of the kernel without the f16 arithmetic, without the logic,
-// the tensor products, the scaling or the exponentials save 4 us at most each,
-// one that only loads takes 61, and one that loads no page still takes 24: the
-// start (a chain of loads of 1 us each to the first page, cold code) and the
-// join of the parts.
+// slower, 88 against 78 us for 273 MB.)  What bounds a call of 74 to 77 us over
+// 273 MB, measured before the weights followed the value scales: copies of the
+// kernel without the f16 arithmetic, without the logic, the tensor products, the
+// scaling or the exponentials save 4 us at most each, one that only loads takes
+// 61, and one that loads no page still takes 24: the start (a chain of loads of
+// 1 us each to the first page, cold code) and the join of the parts.
 template <int NP>
 constexpr int kKv4Warps = NP == 1 ? 12 : 8;
 constexpr int kKv4Rings = 24 * kv4_page_bytes(128);

@@ -62,9 +62,9 @@ inline bool aligned(const void* p, size_t n) { return ((uintptr_t)p % n) == 0; }
 //
 // A row of D codes is W = D/8 words; value d sits in word d % W, nibble
 // nib(d / W).  nib(2p) = p and nib(2p + 1) = p + 4, so that
-// (word >> 8(p/2)) & (0x000f000f << 4(p%2)) is an f16 pair of the values
-// (2p W + w, (2p + 1) W + w), both in one block of 32: the codes read as f16
-// subnormals, code * 2^-24 (2^-20 for odd p), with no conversion.
+// (word >> 8(p/2)) & (0x000f000f << 4(p%2)) has the codes of the values
+// (2p W + w, (2p + 1) W + w), both in one block of 32, in its two halves, as
+// the attention turns them into an f16 pair (an OR and one f16 operation).
 // Tokens of D = 128 whose bit 1 is set hold the two 32-byte halves of a row
 // swapped: the four rows a warp reads at once then lie in different banks.
 // Scales are stored in the order in which the attention's lanes use them:

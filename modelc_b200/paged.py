@@ -268,7 +268,8 @@ def _pool(pool: torch.Tensor, head_dim: int) -> int:
 
 def kv4_append(pool, k, v, slots) -> None:
     """Quantizes k, v [tokens, kv heads, head_dim] into their slots of the
-    pool (q4_0 blocks of 32 values); slots outside the pool are skipped."""
+    pool (q4_0 blocks of 32 values); slots outside the pool are skipped.  No
+    two tokens of one call may share a slot."""
     dev = _pool(pool, k.shape[-1] if k.dim() else 0)
     k, v = _heads(k, "k", dev), _heads(v, "v", dev)
     T, Hk, D = k.shape
@@ -308,7 +309,8 @@ def kv4_attention(q, pool, table, kv_len, cu_q, scale: float | None = None):
     over the cache: rows cu_q[z]..cu_q[z+1] are the last of request z's
     kv_len[z] tokens, which the pool holds already through table [requests,
     width].  ``scale`` is 1/sqrt(head_dim) by default.  Rows that see no key
-    are 0."""
+    are 0.  Weights times value scales are rounded to f16, in bf16 calls the
+    weights too; scores and sums are f32."""
     dev = _gpu(q, "q")
     q = _heads(q, "q", dev)
     T, H, D = q.shape
@@ -342,7 +344,8 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, scale: float | None = None, causa
     """Attention over packed prompts: q [n_q, heads, head_dim], k, v [n_k, kv
     heads, head_dim] (f16, bf16), sequence z holding queries cu_q[z]..cu_q[z+1]
     and keys cu_k[z]..cu_k[z+1] (cu_q's by default).  Causal: its queries are
-    its last tokens.  Rows that see no key are 0."""
+    its last tokens.  Rows that see no key are 0.  Weights are rounded to the
+    inputs' type; scores and sums are f32."""
     dev = _gpu(q, "q")
     q, k, v = _heads(q, "q", dev), _heads(k, "k", dev), _heads(v, "v", dev)
     T, H, D = q.shape
