@@ -1,5 +1,6 @@
 """The workspace of attention over the 4-bit cache: nothing of it stays behind
 a call, and calls that run side by side do not share one."""
+import gc
 import threading
 
 import pytest
@@ -30,8 +31,10 @@ def test_nothing_is_kept():
     import torch
     args = _case(3, 8, 2, 128, 500, 1)
     want = mb.kv4_attention(*args)
+    gc.collect()  # what earlier tests left in cycles
     torch.cuda.synchronize()
-    before = torch.cuda.memory_allocated()
+    torch.cuda.empty_cache()
+    before, reserved = torch.cuda.memory_allocated(), torch.cuda.memory_reserved()
     seen = []
 
     def work():
@@ -49,7 +52,7 @@ def test_nothing_is_kept():
     assert seen == [True] * 10
     assert torch.cuda.memory_allocated() == before
     torch.cuda.empty_cache()
-    assert torch.cuda.memory_reserved() < before + (40 << 20)
+    assert torch.cuda.memory_reserved() <= reserved + (20 << 20)  # one workspace is 19 MB
 
 
 @gpu
